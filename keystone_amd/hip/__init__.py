@@ -14,6 +14,10 @@ Kernels (ref mapping in SURVEY.md §2.9):
   * ``fisher_vector``   — fused GMM-posterior + FV accumulation (K3)
   * ``gmm_posteriors``  — GMM E-step responsibilities (K2)
   * ``sift``            — dense SIFT descriptor family (K1)
+  * ``embedding``       — token lookup, bag sums, the table's gradient by
+                          sorted tokens (``token_sort``)
+  * ``dropout``         — dropout from a counter, its mask never stored
+  * ``fp8_linear``      — 8-bit linear map, a scale for each block of 128
 
 GPU ops FAIL LOUDLY when the extension is missing on a CUDA device — there
 is deliberately no silent eager fallback on GPU (set KEYSTONE_ALLOW_EAGER=1
@@ -26,6 +30,9 @@ import ctypes
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -52,11 +59,28 @@ def build(force: bool = False, arch: str = "gfx950", verbose: bool = True) -> st
                [os.path.join(_SRC, "common.h")]):
             return _LIB_PATH
     hipcc = os.environ.get("HIPCC", "hipcc")
-    cmd = [hipcc, f"--offload-arch={arch}", "-O3", "-std=c++17", "-shared",
-           "-fPIC", "-fvisibility=hidden", "-o", _LIB_PATH] + srcs
+    # packed float32 instructions stay off: some of their forms have given
+    # wrong results on this card
+    cmd = [hipcc, f"--offload-arch={arch}", "-O3", "-std=c++17", "-fPIC",
+           "-fvisibility=hidden", "-Xclang", "-target-feature", "-Xclang",
+           "-packed-fp32-ops"]
     if verbose:
-        print("[keystone_amd.hip] " + " ".join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+        print("[keystone_amd.hip] " + " ".join(cmd + srcs), file=sys.stderr)
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
+
+        def compile_one(src_obj):
+            src, obj = src_obj
+            r = subprocess.run(cmd + ["-c", src, "-o", obj],
+                               stderr=subprocess.PIPE, text=True)
+            if r.returncode:
+                sys.stderr.write(r.stderr)
+                raise subprocess.CalledProcessError(r.returncode, r.args)
+
+        with ThreadPoolExecutor(min(8, len(srcs))) as pool:
+            list(pool.map(compile_one, zip(srcs, objs)))
+        subprocess.run([hipcc, f"--offload-arch={arch}", "-shared", "-fPIC",
+                        "-o", _LIB_PATH] + objs, check=True)
     return _LIB_PATH
 
 
@@ -147,6 +171,33 @@ def _register_extra(lib: ctypes.CDLL) -> None:
         lib.ks_sift_norm2_f32.restype = c_i
     except AttributeError:
         pass
+    c_l, c_u64 = ctypes.c_longlong, ctypes.c_ulonglong
+    try:
+        lib.ks_embedding_lookup.argtypes = [c_p, c_i, c_l, c_p, c_i, c_l, c_l,
+                                            c_p, c_i, c_f, c_i, c_p]
+        lib.ks_embedding_lookup.restype = c_i
+        lib.ks_segment_long.argtypes = []
+        lib.ks_segment_long.restype = c_i
+        lib.ks_segment_sum.argtypes = [
+            c_i, c_p, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_p, c_p, c_i,
+            c_l, c_p, c_i, c_l, c_p, c_i, c_f, c_i, c_i, c_p]
+        lib.ks_segment_sum.restype = c_i
+        lib.ks_token_sort_work.argtypes = [c_i, c_i]
+        lib.ks_token_sort_work.restype = c_l
+        lib.ks_token_sort.argtypes = [c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_i,
+                                      c_p, c_p, c_p, c_p, c_p, c_p]
+        lib.ks_token_sort.restype = c_i
+        lib.ks_dropout.argtypes = [c_p, c_p, c_l, c_i, ctypes.c_uint, c_f,
+                                   c_u64, c_u64, c_p, c_p]
+        lib.ks_dropout.restype = c_i
+        lib.ks_fp8_quantise.argtypes = [c_p, c_i, c_l, c_i, c_i, c_p, c_p, c_p]
+        lib.ks_fp8_quantise.restype = c_i
+        lib.ks_fp8_splits.argtypes = [c_i, c_i, c_i]
+        lib.ks_fp8_splits.restype = c_i
+        lib.ks_fp8_gemm.argtypes = [c_p] * 6 + [c_i, c_p, c_i, c_i, c_i, c_p]
+        lib.ks_fp8_gemm.restype = c_i
+    except AttributeError:
+        pass
 
 
 def available() -> bool:
@@ -175,6 +226,25 @@ def gpu_ready() -> bool:
 
 def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _raw_stream(device: torch.device) -> int:
+    """The current stream of ``device``."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+_NO_GUARD = nullcontext()
+
+
+def _guard(device: torch.device):
+    """Makes ``device`` current for a launch, where it is not."""
+    if device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _check(code: int, name: str) -> None:
@@ -634,3 +704,9 @@ def sym_rectify(X: torch.Tensor, alpha: float = 0.0) -> torch.Tensor:
         ctypes.c_void_p(X.data_ptr()), ctypes.c_void_p(out.data_ptr()),
         rows, cols, alpha, _stream()), "ks_sym_rectify_f32")
     return out
+
+
+from .counter_dropout import dropout, dropout_threshold  # noqa: E402
+from .embedding import (EmbeddingPlan, embedding_bag,  # noqa: E402
+                        embedding_grad, embedding_lookup, embedding_plan)
+from .fp8 import Fp8Weight, fp8_linear, fp8_pack, fp8_round  # noqa: E402

@@ -1,0 +1,95 @@
+// Dropout from a counter: whether element i of a call is kept is a function
+// of (seed, step, i) alone, so no mask is stored and the gradient's pass is
+// the forward pass on the gradient.
+//
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as
+// easy as 1, 2, 3", 2011) with key = seed and counter = (i div 8, step): its
+// four 32-bit words are eight 16-bit numbers, one for each of eight
+// neighbours.  An element is kept where its number is at least
+// t = round(65536 p), so that the chance is exact to 2^-16, and a kept one is
+// scaled by 65536 / (65536 - t), the inverse of the chance that is meant by
+// t: the mean stays exact.  One rounding, to the output's type.
+#include "common.h"
+
+#include <cstdint>
+
+namespace {
+
+__device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0,
+                                       uint32_t k1) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t a = (uint64_t)c[0] * 0xD2511F53u;
+        const uint64_t b = (uint64_t)c[2] * 0xCD9E8D57u;
+        c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
+        c[1] = (uint32_t)b;
+        c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
+        c[3] = (uint32_t)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+}
+
+// WIDE: both arrays begin on 16 bytes.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256)
+void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long long n,
+                    uint32_t threshold, float scale, uint64_t seed,
+                    uint64_t step, const long long* __restrict__ step_at) {
+    using V8 = T __attribute__((ext_vector_type(8)));
+    if (step_at) step = (uint64_t)*step_at;
+    const long long blocks = (n + 7) / 8;
+    for (long long b = (long long)blockIdx.x * 256 + threadIdx.x; b < blocks;
+         b += (long long)gridDim.x * 256) {
+        uint32_t c[4] = {(uint32_t)b, (uint32_t)((uint64_t)b >> 32),
+                         (uint32_t)step, (uint32_t)(step >> 32)};
+        philox(c, (uint32_t)seed, (uint32_t)(seed >> 32));
+        const long long i = b * 8;
+        if (WIDE && i + 8 <= n) {
+            V8 v = *reinterpret_cast<const V8*>(x + i);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t r = k & 1 ? c[k >> 1] >> 16 : c[k >> 1] & 0xffffu;
+                v[k] = r >= threshold ? (T)((float)v[k] * scale) : (T)0.0f;
+            }
+            *reinterpret_cast<V8*>(y + i) = v;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t r = k & 1 ? c[k >> 1] >> 16 : c[k >> 1] & 0xffffu;
+                if (i + k < n)
+                    y[i + k] = r >= threshold ? (T)((float)x[i + k] * scale)
+                                              : (T)0.0f;
+            }
+        }
+    }
+}
+
+template <typename T>
+int dropout(const void* x, void* y, long long n, uint32_t threshold,
+            float scale, uint64_t seed, uint64_t step, const long long* step_at,
+            hipStream_t stream) {
+    long long grid = ((n + 7) / 8 + 255) / 256;
+    if (grid > 256 * 16) grid = 256 * 16;
+    const bool wide = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
+    auto* kernel = wide ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+    kernel<<<(unsigned)grid, 256, 0, stream>>>((const T*)x, (T*)y, n, threshold,
+                                               scale, seed, step, step_at);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+// y = dropout(x) over n elements; type 0: float32, 1: bfloat16, 2: float16.
+// step_at: the step in device memory; null: `step`.
+KS_EXPORT int ks_dropout(const void* x, void* y, long long n, int type,
+                         unsigned threshold, float scale,
+                         unsigned long long seed, unsigned long long step,
+                         const long long* step_at, hipStream_t stream) {
+    if (n == 0) return 0;
+    switch (type) {
+        case 0: return dropout<float>(x, y, n, threshold, scale, seed, step, step_at, stream);
+        case 1: return dropout<__bf16>(x, y, n, threshold, scale, seed, step, step_at, stream);
+        default: return dropout<_Float16>(x, y, n, threshold, scale, seed, step, step_at, stream);
+    }
+}

@@ -1,0 +1,311 @@
+// Y = X W + b with both operands in e4m3 and a scale for every 128 of the
+// inner dimension.
+//
+// A block of 128 neighbours along K of a row of X (a column of W) is held as
+// q 2^e with q in e4m3 and e the least exponent that brings the block under
+// 448, the type's largest.  A power of two makes the scaling itself exact,
+// so that the only rounding is q's own, at most 2^-4 of the value, and it is
+// the scale that v_mfma_scale_f32_16x16x128_f8f6f4 applies by itself to 128
+// products at a time: the accumulator never leaves the matrix unit.
+//
+// Both operands lie in memory as the matrix instruction takes them: 16 rows
+// by 128 of K are one chunk of 2048 bytes, two planes of 16 bytes a lane, so
+// that every load is a whole line and no operand is moved between lanes.
+// Byte t of lane l is element k = 32 (t div 8) + 8 (l div 16) + t mod 8 of
+// row l mod 16: an order of K that quantising reads in whole sectors.  Rows
+// past the end and K past the end are zeros.
+#include "common.h"
+
+#include <cstdint>
+
+namespace {
+
+using i32x4 = int __attribute__((ext_vector_type(4)));
+using i32x8 = int __attribute__((ext_vector_type(8)));
+
+constexpr int CHUNK = 2048;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool wide, int left,
+                                      float (&v)[8]) {
+    using V4 = T __attribute__((ext_vector_type(16 / sizeof(T))));
+    if (wide && left >= 8) {
+        constexpr int W = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < 8 / W; ++q) {
+            const V4 x = reinterpret_cast<const V4*>(p)[q];
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[q * W + k] = (float)x[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k < left ? (float)p[k] : 0.0f;
+    }
+}
+
+// One wave a chunk: 16 rows by 128 of K.  scales[tile][K/512][16] has a
+// byte, 127 + e, for each of four blocks.
+template <typename T>
+__global__ __launch_bounds__(256)
+void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
+                         int K, int tiles, int kblocks, int wide,
+                         unsigned char* __restrict__ q,
+                         unsigned char* __restrict__ scales) {
+    const long long chunk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (chunk >= (long long)tiles * kblocks) return;
+    const int kb = (int)(chunk % kblocks), tile = (int)(chunk / kblocks);
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const int row = tile * 16 + (lane & 15);
+    float v[4][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int k = kb * 128 + j * 32 + g * 8;
+        load8(x + (long long)row * ld + k, wide && row < rows,
+              row < rows ? K - k : 0, v[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    // top = m 2^p with m in [1, 2); 448 = 1.75 2^8
+    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u);
+    const bool bad = top >= 0x7f800000u;
+    if (top == 0 || bad) e = 0;
+    if (e < -117) e = -117;
+    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int d = 0;
+            d = __builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * h] * inv,
+                                                v[j][4 * h + 1] * inv, d, false);
+            d = __builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * h + 2] * inv,
+                                                v[j][4 * h + 3] * inv, d, true);
+            // a block that holds an infinity or a NaN is NaN throughout
+            w[2 * j + h] = bad ? 0x7f7f7f7fu : (uint32_t)d;
+        }
+    }
+    unsigned char* to = q + chunk * CHUNK + lane * 16;
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(to + 1024) = make_uint4(w[4], w[5], w[6], w[7]);
+    if (lane < 16)
+        scales[((long long)tile * ((kblocks + 3) / 4) + kb / 4) * 64 +
+               lane * 4 + (kb & 3)] = (unsigned char)(127 + e);
+}
+
+struct Gemm {
+    const unsigned char* xq;   // activations: [tiles of M][K/128] chunks
+    const unsigned* xs;        // [tiles of M][K/512][16]
+    const unsigned char* wq;   // weights: [tiles of N][K/128] chunks
+    const unsigned* ws;
+    int M, N, kblocks;
+};
+
+__device__ __forceinline__ i32x8 load_chunk(const unsigned char* base, int lane) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(base + lane * 16);
+    const i32x4 hi = *reinterpret_cast<const i32x4*>(base + 1024 + lane * 16);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+
+// Eight bytes times 2^e, exactly; scale: 127 + e.
+__device__ __forceinline__ bf16x8 widen(int lo, int hi, int scale) {
+    const float s = __uint_as_float((uint32_t)scale << 23);
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// acc += (16 rows of W) (16 rows of X)^T over 128 of K: lane l gets columns
+// n = 4 (l div 16) + 0..3 of row m = l mod 16.
+__device__ __forceinline__ f32x4 mfma(i32x8 w, i32x8 x, f32x4 acc, int ws,
+                                      int xs) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+        w, x, acc, 0, 0, 0, ws, 0, xs);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
+                                              int N, bool wide, f32x4 v,
+                                              const float* bias) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (bias && n + k < N) v[k] += bias[n + k];
+    T* to = y + m * ld + n;
+    if (wide && n + 4 <= N) {
+        using V4 = T __attribute__((ext_vector_type(4)));
+        V4 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
+        *reinterpret_cast<V4*>(to) = o;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (n + k < N) to[k] = (T)v[k];
+    }
+}
+
+// A wave has TM x TN tiles of 16 x 16; its operands come straight from
+// memory.  Split s of gridDim.z takes K blocks [s kper, (s + 1) kper); with
+// more than one split, `part` [splits][M][N] takes the sums.
+// EXACT: products and sums for 32-bit outputs.
+template <typename T, int TM, int TN, bool EXACT>
+__global__ __launch_bounds__(256)
+void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
+                     const float* __restrict__ bias, int wide, int kper) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int mtiles = ks_ceil_div(a.M, 16), ntiles = ks_ceil_div(a.N, 16);
+    const int m0 = blockIdx.y * TM, n0 = (blockIdx.x * 4 + wave) * TN;
+    if (n0 >= ntiles) return;
+    const int k0 = blockIdx.z * kper, k1 = min(a.kblocks, k0 + kper);
+    const int kq = (a.kblocks + 3) / 4;
+    f32x4 acc[TM][TN] = {};
+    for (int kb = k0; kb < k1; ++kb) {
+        i32x8 xf[TM], wf[TN];
+        int xs[TM], ws[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int t = min(m0 + i, mtiles - 1);
+            xf[i] = load_chunk(a.xq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
+            xs[i] = (int)(a.xs[((long long)t * kq + kb / 4) * 16 + (lane & 15)]
+                          >> (8 * (kb & 3))) & 255;
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int t = min(n0 + j, ntiles - 1);
+            wf[j] = load_chunk(a.wq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
+            ws[j] = (int)(a.ws[((long long)t * kq + kb / 4) * 16 + (lane & 15)]
+                          >> (8 * (kb & 3))) & 255;
+        }
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                bf16x8 x[TM], w[TN];
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                    x[i] = widen(xf[i][2 * s], xf[i][2 * s + 1], xs[i]);
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    w[j] = widen(wf[j][2 * s], wf[j][2 * s + 1], ws[j]);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            w[j], x[i], acc[i][j], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = mfma(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int m = (m0 + i) * 16 + (lane & 15);
+            const int n = (n0 + j) * 16 + (lane >> 4) * 4;
+            if (m >= a.M || n >= a.N) continue;
+            if (part)
+                store_columns<float>(part + (long long)blockIdx.z * a.M * a.N,
+                                     a.N, m, n, a.N, a.N % 4 == 0, acc[i][j],
+                                     nullptr);
+            else
+                store_columns<T>(y, a.N, m, n, a.N, wide, acc[i][j], bias);
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void fp8_join_kernel(const float* __restrict__ part, int splits, long long n,
+                     int N, const float* __restrict__ bias, T* __restrict__ y) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n;
+         i += (long long)gridDim.x * 256) {
+        float s = 0.0f;
+        for (int k = 0; k < splits; ++k) s += part[k * n + i];
+        if (bias) s += bias[i % N];
+        y[i] = (T)s;
+    }
+}
+
+template <typename T>
+int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
+             unsigned char* scales, hipStream_t stream) {
+    const int tiles = ks_ceil_div(rows, 16), kblocks = ks_ceil_div(K, 128);
+    const int wide = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
+    const long long chunks = (long long)tiles * kblocks;
+    fp8_quantise_kernel<T><<<(unsigned)((chunks + 3) / 4), 256, 0, stream>>>(
+        (const T*)x, ld, rows, K, tiles, kblocks, wide, q, scales);
+    return (int)hipGetLastError();
+}
+
+// How many ways K is split: enough waves to fill the card.
+int splits_of(int M, int N, int kblocks) {
+    const long long blocks = (long long)ks_ceil_div(M, 64) * ks_ceil_div(N, 256);
+    long long s = 512 / blocks;
+    if (s > kblocks / 4) s = kblocks / 4;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <typename T>
+int gemm(const Gemm& a, void* y, float* part, const float* bias, int splits,
+         hipStream_t stream) {
+    const int wide = a.N % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
+    const int kper = ks_ceil_div(a.kblocks, splits);
+    const dim3 grid(ks_ceil_div(a.N, 256), ks_ceil_div(a.M, 64), splits);
+    fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4><<<grid, 256, 0, stream>>>(
+        a, (T*)y, splits > 1 ? part : nullptr, bias, wide, kper);
+    if (splits > 1) {
+        const long long n = (long long)a.M * a.N;
+        long long blocks = (n + 255) / 256;
+        if (blocks > 2048) blocks = 2048;
+        fp8_join_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(
+            part, splits, n, a.N, bias, (T*)y);
+    }
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+// q: 16 ceil(rows/16) x 128 ceil(K/128) bytes, scales: 64 bytes for every 16
+// rows and 512 of K; type 0: float32, 1: bfloat16, 2: float16.
+KS_EXPORT int ks_fp8_quantise(const void* x, int type, long long ld, int rows,
+                              int K, unsigned char* q, unsigned char* scales,
+                              hipStream_t stream) {
+    if (rows == 0 || K == 0) return 0;
+    switch (type) {
+        case 0: return quantise<float>(x, ld, rows, K, q, scales, stream);
+        case 1: return quantise<__bf16>(x, ld, rows, K, q, scales, stream);
+        default: return quantise<_Float16>(x, ld, rows, K, q, scales, stream);
+    }
+}
+
+// How many [M, N] float32 parts ks_fp8_gemm needs; 1: none.
+KS_EXPORT int ks_fp8_splits(int M, int N, int K) {
+    return splits_of(M, N, ks_ceil_div(K, 128));
+}
+
+KS_EXPORT int ks_fp8_gemm(const unsigned char* xq, const unsigned* xs,
+                          const unsigned char* wq, const unsigned* ws,
+                          const float* bias, void* y, int type, float* part,
+                          int M, int K, int N, hipStream_t stream) {
+    if (M == 0 || N == 0) return 0;
+    const Gemm a{xq, xs, wq, ws, M, N, ks_ceil_div(K, 128)};
+    const int s = splits_of(M, N, a.kblocks);
+    switch (type) {
+        case 0: return gemm<float>(a, y, part, bias, s, stream);
+        case 1: return gemm<__bf16>(a, y, part, bias, s, stream);
+        default: return gemm<_Float16>(a, y, part, bias, s, stream);
+    }
+}
