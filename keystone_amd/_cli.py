@@ -18,6 +18,9 @@ def main():
     ng.add_argument("--num-classes", type=int, default=20)
     ng.add_argument("--common-features", type=int, default=20000)
     ng.add_argument("--data-dir", help="dir-per-class text corpus")
+    ng.add_argument("--features", choices=["ngrams", "embedding"],
+                    default="ngrams", help="counted n-grams with naive "
+                    "Bayes, or learned word embeddings")
 
     am = sub.add_parser("amazon")
     am.add_argument("--n-docs", type=int, default=2000)
@@ -32,6 +35,8 @@ def main():
     tm.add_argument("--n", type=int, default=50000)
     tm.add_argument("--num-features", type=int, default=8192)
     tm.add_argument("--epochs", type=int, default=3)
+    tm.add_argument("--fp8-scores", action="store_true",
+                    help="score with 8-bit class weights and features")
 
     cf = sub.add_parser("cifar")
     cf.add_argument("--n", type=int, default=2000)
@@ -50,6 +55,8 @@ def main():
     im.add_argument("--num-classes", type=int, default=1000)
     im.add_argument("--gmm-k", type=int, default=64)
     im.add_argument("--save", help="save the fitted pipeline here")
+    im.add_argument("--fp8-scores", action="store_true",
+                    help="score with 8-bit class weights and features")
     im.add_argument("--solver-checkpoint", help="epoch checkpoint dir "
                     "(re-run with the same dir to resume the solver)")
 
@@ -62,15 +69,23 @@ def main():
     if args.app == "newsgroups":
         from keystone_amd.evaluation import MulticlassClassifierEvaluator
         from keystone_amd.loaders import NewsgroupsDataLoader, synthetic_documents
-        from keystone_amd.models import NewsgroupsConfig, build_newsgroups
+        from keystone_amd.models import (NewsgroupsConfig,
+                                         NewsgroupsEmbeddingConfig,
+                                         build_newsgroups,
+                                         build_newsgroups_embedding)
         if args.data_dir:
             docs, labels, classes = NewsgroupsDataLoader(args.data_dir)
             k = len(classes)
         else:
             docs, labels = synthetic_documents(args.n_docs, args.num_classes)
             k = args.num_classes
-        pipe = build_newsgroups(docs, labels, NewsgroupsConfig(
-            num_classes=k, common_features=args.common_features))
+        if args.features == "embedding":
+            pipe = build_newsgroups_embedding(
+                docs, labels, NewsgroupsEmbeddingConfig(
+                    num_classes=k, num_words=args.common_features))
+        else:
+            pipe = build_newsgroups(docs, labels, NewsgroupsConfig(
+                num_classes=k, common_features=args.common_features))
         m = MulticlassClassifierEvaluator(k).evaluate(pipe.apply(docs), labels)
         if rt.rank == 0:
             print(f"train {m.summary()}  ({time.time()-t0:.1f}s)")
@@ -109,7 +124,8 @@ def main():
         from keystone_amd.models import TimitConfig, build_timit
         train, labels = synthetic_timit(args.n)
         pipe = build_timit(train, labels, TimitConfig(
-            num_features=args.num_features, num_iter=args.epochs))
+            num_features=args.num_features, num_iter=args.epochs,
+            fp8_scores=args.fp8_scores))
         m = MulticlassClassifierEvaluator(147).evaluate(pipe.apply(train), labels)
         if rt.rank == 0:
             print(f"train {m.summary()}  ({time.time()-t0:.1f}s)")
@@ -173,6 +189,7 @@ def main():
                                         num_classes=args.num_classes)
         conf = ImageNetFVConfig(num_classes=args.num_classes,
                                 gmm_k=args.gmm_k,
+                                fp8_scores=args.fp8_scores,
                                 solver_checkpoint_dir=args.solver_checkpoint)
         pipe, info = fit_imagenet_fv(imgs, labels, conf)
         if args.save:

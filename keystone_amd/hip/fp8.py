@@ -105,6 +105,9 @@ def _quantise(lib, x: torch.Tensor):
 
 def fp8_pack(W: torch.Tensor) -> Fp8Weight:
     """Quantises a [K, N] weight matrix and lays it out, once."""
+    if W.dim() != 2:
+        raise ValueError(f"fp8_pack.W: expected a matrix, got shape "
+                         f"{tuple(W.shape)}")
     if W.is_cuda:
         lib = _load()
         W = _operand(W.t(), "fp8_pack.W")

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-from ..ops.learning import BlockLeastSquaresEstimator
+from ..ops.learning import BlockLeastSquaresEstimator, QuantizedEstimator
 from ..ops.stats import (CosineRandomFeatures, PaddedFFT, RandomSignNode,
                          StandardScaler)
 from ..ops.util import (ClassLabelIndicatorsFromIntLabels, MaxClassifier,
@@ -74,6 +74,8 @@ class TimitConfig:
     num_iter: int = 3
     lam: float = 1e-3
     seed: int = 0
+    # scores with class weights and features in 8 bits
+    fp8_scores: bool = False
 
 
 def build_timit(train, labels_int, conf: TimitConfig = TimitConfig()
@@ -81,10 +83,12 @@ def build_timit(train, labels_int, conf: TimitConfig = TimitConfig()
     ind = ClassLabelIndicatorsFromIntLabels(conf.num_classes)
     labels = TensorDataset(ind.apply_batch(labels_int.data).float(),
                            labels_int.runtime)
+    solver = BlockLeastSquaresEstimator(conf.block_size, conf.num_iter,
+                                        conf.lam)
+    if conf.fp8_scores:
+        solver = QuantizedEstimator(solver)
     return (StandardScaler().with_data(train)
             .and_then(CosineRandomFeatures(conf.input_dim, conf.num_features,
                                            conf.gamma, seed=conf.seed))
-            .and_then(BlockLeastSquaresEstimator(conf.block_size,
-                                                 conf.num_iter, conf.lam),
-                      train, labels)
+            .and_then(solver, train, labels)
             .and_then(MaxClassifier()))

@@ -63,6 +63,8 @@ class ImageNetFVConfig:
     seed: int = 0
     gmm_iters: int = 20
     kmeans_iters: int = 5
+    # the inference pipeline scores with class weights and features in 8 bits
+    fp8_scores: bool = False
 
 
 def _fit_branch(extractor: PipelineBase, train_imgs: TensorDataset,
@@ -161,7 +163,7 @@ def fit_imagenet_fv(train_imgs: TensorDataset, labels_int: TensorDataset,
     info["model"] = model
 
     pipe = (gather(branches).and_then(VectorCombiner())
-            .and_then(model)
+            .and_then(model.quantize() if conf.fp8_scores else model)
             .and_then(TopKClassifier(min(conf.top_k, conf.num_classes))))
     info["t_total"] = time.perf_counter() - t0
     return pipe, info

@@ -13,9 +13,11 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-from ..ops.learning import LogisticRegressionEstimator, NaiveBayesEstimator
+from ..ops.learning import (EmbeddingClassifierEstimator,
+                            LogisticRegressionEstimator, NaiveBayesEstimator)
 from ..ops.nlp import (CommonSparseFeatures, LowerCase, NGramsFeaturizer,
-                       TermFrequency, Tokenizer, Trim)
+                       PadTokens, TermFrequency, Tokenizer, Trim,
+                       WordFrequencyEncoder)
 from ..ops.util import MaxClassifier
 from ..workflow.pipeline import Pipeline
 
@@ -40,6 +42,37 @@ def build_newsgroups(train_docs, train_labels,
             .and_then(CommonSparseFeatures(conf.common_features), train_docs)
             .and_then(NaiveBayesEstimator(conf.num_classes), train_docs,
                       train_labels)
+            .and_then(MaxClassifier()))
+
+
+@dataclass
+class NewsgroupsEmbeddingConfig:
+    num_classes: int = 20
+    num_words: int = 20000
+    doc_len: int = 256
+    dim: int = 64
+    num_epochs: int = 5
+    batch_size: int = 256
+    step_size: float = 1.0
+    dropout: float = 0.1
+    seed: int = 0
+
+
+def build_newsgroups_embedding(
+        train_docs, train_labels,
+        conf: NewsgroupsEmbeddingConfig = NewsgroupsEmbeddingConfig()
+        ) -> Pipeline:
+    """Trim -> LowerCase -> Tokenizer -> WordFrequencyEncoder -> PadTokens ->
+    EmbeddingClassifier -> MaxClassifier: learned word embeddings in the
+    place of counted n-grams."""
+    words = Trim().and_then(LowerCase()).and_then(Tokenizer())
+    return (words
+            .and_then(WordFrequencyEncoder(), train_docs)
+            .and_then(PadTokens(conf.doc_len))
+            .and_then(EmbeddingClassifierEstimator(
+                conf.num_words, conf.num_classes, conf.dim, conf.num_epochs,
+                conf.batch_size, conf.step_size, conf.dropout, conf.seed),
+                train_docs, train_labels)
             .and_then(MaxClassifier()))
 
 

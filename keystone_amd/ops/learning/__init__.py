@@ -14,6 +14,9 @@ from .whitening import ZCAWhitener, ZCAWhitenerEstimator, LinearDiscriminantAnal
 from .krr import (GaussianKernelGenerator, KernelRidgeRegression,
                   KernelBlockLinearMapper)
 from .kernel_matrix import KernelMatrix, BlockKernelMatrix
+from .quantized import QuantizedEstimator, QuantizedLinearMapper
+from .embedding_classifier import (EmbeddingClassifierEstimator,
+                                   EmbeddingClassifierModel)
 
 __all__ = [
     "LinearMapper", "LinearMapEstimator", "LocalLeastSquaresEstimator",
@@ -30,4 +33,6 @@ __all__ = [
     "ZCAWhitener", "ZCAWhitenerEstimator", "LinearDiscriminantAnalysis",
     "GaussianKernelGenerator", "KernelRidgeRegression",
     "KernelBlockLinearMapper", "KernelMatrix", "BlockKernelMatrix",
+    "QuantizedLinearMapper", "QuantizedEstimator",
+    "EmbeddingClassifierEstimator", "EmbeddingClassifierModel",
 ]

@@ -104,6 +104,16 @@ class BlockLinearMapper(Transformer):
             return ds.map_batch(self.apply_batch)
         return ds.map(self.apply)
 
+    def quantize(self):
+        """The same map with 8-bit weights, for serving: on the blocks' joint
+        features."""
+        from .quantized import QuantizedLinearMapper
+        if self.featurizers is not None:
+            raise ValueError("a map with lazy featurizers never has its "
+                             "features whole: it cannot be quantized")
+        return QuantizedLinearMapper.from_weights(torch.cat(self.blocks),
+                                                  self.intercept)
+
     # persistence: store blocks as stacked state
     def get_state(self):
         st = {f"block_{i}": b for i, b in enumerate(self.blocks)}

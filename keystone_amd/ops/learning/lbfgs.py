@@ -18,7 +18,9 @@ import torch
 
 from ...parallel.dataset import TensorDataset
 from ...workflow.pipeline import LabelEstimator
+from ..stats.dropout import dropout
 from .linear import LinearMapper
+from .sparse_rows import SparseRows
 
 __all__ = ["LeastSquaresGradient", "LogisticGradient", "DenseLBFGSwithL2",
            "SparseLBFGSwithL2", "MiniBatchSGDwithL2"]
@@ -57,6 +59,8 @@ class LogisticGradient(Gradient):
 
 def _xt_mm(X: torch.Tensor, D: torch.Tensor) -> torch.Tensor:
     """X^T @ D for dense or sparse-CSR X."""
+    if isinstance(X, SparseRows):
+        return X.t_matmul(D)
     if X.layout == torch.sparse_csr or X.is_sparse:
         # CSR has no cheap transpose-matmul; go through COO transpose
         return torch.sparse.mm(X.to_sparse_coo().t(), D)
@@ -88,7 +92,11 @@ class _LBFGSBase(LabelEstimator):
         Y = Y.to(dtype)
         rt = data.runtime
         d = X.shape[1] + (1 if self.fit_intercept else 0)
-        if self.fit_intercept:
+        # a user's own gradient gets X as the tensor that it is
+        if type(self.gradient) in (LeastSquaresGradient, LogisticGradient) \
+                and SparseRows.supports(X):
+            X = SparseRows(X, self.fit_intercept)
+        elif self.fit_intercept:
             ones = torch.ones(X.shape[0], 1, dtype=dtype, device=Y.device)
             X = torch.cat([X.to_dense() if X.layout == torch.sparse_csr else X,
                            ones], dim=1)
@@ -173,7 +181,9 @@ class DenseLBFGSwithL2(_LBFGSBase):
 
 class SparseLBFGSwithL2(_LBFGSBase):
     """ref: SparseLBFGSwithL2 — X as torch sparse CSR; gradient GEMMs go
-    through sparse kernels (rocSPARSE via torch on ROCm)."""
+    through sparse kernels: on the GPU float32 rows through the embedding
+    kernels (``SparseRows``, columns sorted once a fit), else rocSPARSE via
+    torch."""
 
     def _prepare(self, X):
         if X.layout != torch.sparse_csr and not X.is_sparse:
@@ -183,11 +193,15 @@ class SparseLBFGSwithL2(_LBFGSBase):
 
 class MiniBatchSGDwithL2(LabelEstimator):
     """ref (SURVEY.md §2.2 [L]): MiniBatchSGDwithL2 — synchronous SGD with
-    per-step all-reduced gradients."""
+    per-step all-reduced gradients.  ``dropout``: the chance that a step
+    leaves out a feature of a row (the kept ones are scaled up), which for
+    linear models is a regulariser fitted to the features' scales."""
 
     def __init__(self, gradient: Gradient, num_iterations: int = 100,
                  step_size: float = 0.1, batch_fraction: float = 0.1,
-                 reg_param: float = 0.0, seed: int = 0):
+                 reg_param: float = 0.0, seed: int = 0,
+                 dropout: float = 0.0):
+        self.dropout = dropout
         self.gradient = gradient
         self.num_iterations = num_iterations
         self.step_size = step_size
@@ -208,7 +222,10 @@ class MiniBatchSGDwithL2(LabelEstimator):
         bs = max(1, int(n_local * self.batch_fraction))
         for it in range(self.num_iterations):
             idx = torch.randperm(n_local, generator=g)[:bs].to(X.device)
-            _loss, grad = self.gradient.compute(W, X[idx], Y[idx])
+            Xb = X[idx]
+            if self.dropout:
+                Xb = dropout(Xb, self.dropout, self.seed + 7919 * rt.rank, it)
+            _loss, grad = self.gradient.compute(W, Xb, Y[idx])
             grad = grad.to(torch.float64)
             rt.all_reduce_(grad)
             grad = grad.to(X.dtype) / (bs * rt.world_size)

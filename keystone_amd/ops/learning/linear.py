@@ -91,6 +91,11 @@ class LinearMapper(BatchTransformer):
             out = out + self.b
         return out
 
+    def quantize(self):
+        """The same map with 8-bit weights, for serving."""
+        from .quantized import QuantizedLinearMapper
+        return QuantizedLinearMapper.from_weights(self.W, self.b)
+
     @classmethod
     def from_saved(cls, config, state):
         return cls(state["W"], state.get("b"))

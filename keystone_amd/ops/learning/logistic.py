@@ -14,6 +14,7 @@ from ...parallel.dataset import TensorDataset
 from ...workflow.pipeline import BatchTransformer, LabelEstimator
 from .lbfgs import DenseLBFGSwithL2, LogisticGradient, SparseLBFGSwithL2
 from .linear import LinearMapper
+from .sparse_rows import SparseRows
 
 __all__ = ["LogisticRegressionEstimator", "LogisticRegressionModel",
            "NaiveBayesEstimator", "NaiveBayesModel"]
@@ -31,7 +32,12 @@ class LogisticRegressionModel(BatchTransformer):
 
     def apply_batch(self, X: torch.Tensor) -> torch.Tensor:
         self.W = self.W.to(device=X.device, dtype=X.dtype if X.dtype.is_floating_point else self.W.dtype)
-        S = X @ self.W
+        if SparseRows.supports(X):
+            from ... import hip
+            S = hip.embedding_bag(self.W, X.col_indices(), X.crow_indices(),
+                                  X.values())
+        else:
+            S = X @ self.W
         if self.b is not None:
             self.b = self.b.to(device=X.device, dtype=self.W.dtype)
             S = S + self.b
@@ -80,6 +86,11 @@ class NaiveBayesModel(BatchTransformer):
         self.log_theta = self.log_theta.to(device=X.device)
         self.log_prior = self.log_prior.to(device=X.device)
         lt, lp = self.log_theta, self.log_prior
+        if SparseRows.supports(X):
+            from ... import hip
+            return hip.embedding_bag(lt.to(X.dtype), X.col_indices(),
+                                     X.crow_indices(), X.values()
+                                     ) + lp.to(X.dtype)
         if X.layout == torch.sparse_csr or X.is_sparse:
             return torch.sparse.mm(X, lt.to(X.dtype)) + lp.to(X.dtype)
         return X @ lt.to(X.dtype) + lp.to(X.dtype)

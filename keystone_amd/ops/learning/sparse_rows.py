@@ -1,0 +1,52 @@
+"""CSR rows as the iterative solvers multiply by them on the GPU.
+
+With a row's column indices as the tokens of a bag and its values as their
+weights, ``X @ W`` is a sum of W's rows over bags and ``X.T @ D`` the gradient
+of such a sum, by columns sorted once for the whole fit.  An intercept is a
+column of ones that is never stored.
+"""
+
+from __future__ import annotations
+
+import torch
+
+__all__ = ["SparseRows"]
+
+
+class SparseRows:
+    """float32 CSR rows [n, d] on the GPU, with ``intercept`` [n, d + 1]."""
+
+    def __init__(self, csr: torch.Tensor, intercept: bool = False):
+        from ... import hip
+        self.hip = hip
+        self.offsets = csr.crow_indices()
+        self.columns = csr.col_indices()
+        self.values = csr.values()
+        self.intercept = intercept
+        self.features = csr.shape[1]
+        self.shape = torch.Size((csr.shape[0], csr.shape[1] + intercept))
+        self.plan = hip.embedding_plan(self.columns, self.features,
+                                       self.offsets)
+
+    @staticmethod
+    def supports(X: torch.Tensor) -> bool:
+        if not (X.layout == torch.sparse_csr and X.is_cuda
+                and X.dtype == torch.float32):
+            return False
+        from ... import hip
+        return hip.gpu_ready()
+
+    def __matmul__(self, W: torch.Tensor) -> torch.Tensor:
+        S = self.hip.embedding_bag(W[:self.features], self.columns,
+                                   self.offsets, self.values)
+        return S + W[self.features] if self.intercept else S
+
+    def t_matmul(self, D: torch.Tensor) -> torch.Tensor:
+        """``X.T @ D``."""
+        out = torch.empty(self.shape[1], D.shape[1], dtype=torch.float32,
+                          device=D.device)
+        self.hip.embedding_grad(D, self.plan, self.values,
+                                out=out[:self.features])
+        if self.intercept:
+            out[self.features] = D.sum(0)
+        return out

@@ -3,6 +3,7 @@ from .ngrams import NGram, NGramsFeaturizer, NGramsCounts
 from .termfreq import TermFrequency
 from .vocab import (CommonSparseFeatures, SparseFeatureVectorizer,
                     WordFrequencyEncoder)
+from .embedding import MeanEmbedding, PadTokens, TokenEmbedding
 from .backoff_lm import NGramIndexer, StupidBackoffEstimator, StupidBackoffModel
 
 __all__ = [
@@ -10,4 +11,5 @@ __all__ = [
     "NGramsCounts", "TermFrequency", "CommonSparseFeatures",
     "SparseFeatureVectorizer", "WordFrequencyEncoder",
     "StupidBackoffEstimator", "StupidBackoffModel", "NGramIndexer",
+    "PadTokens", "TokenEmbedding", "MeanEmbedding",
 ]

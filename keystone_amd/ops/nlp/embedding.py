@@ -1,0 +1,143 @@
+"""Token embeddings: rows of a table by word id, and their means.
+
+The ids are WordFrequencyEncoder's frequency ranks (ref:
+nodes.nlp.WordFrequencyEncoder), -1 for an unseen word.  An id outside the
+table stands for no word: zeros from a lookup, no term of a mean, no
+gradient.  On the GPU these run as the kernels of ``keystone_amd.hip``; the
+CPU path is plain torch and differentiates nothing by itself either.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from ...parallel.dataset import Dataset, TensorDataset
+from ...workflow.pipeline import BatchTransformer, Transformer
+
+__all__ = ["PadTokens", "TokenEmbedding", "MeanEmbedding", "embed_tokens",
+           "sum_tokens", "token_table_grad", "mean_weights"]
+
+
+def _hip(t: torch.Tensor):
+    """The kernels, where t's device and type go through them."""
+    if t.is_cuda and t.dtype in (torch.float32, torch.bfloat16,
+                                 torch.float16):
+        from ... import hip
+        if hip.gpu_ready():
+            return hip
+    return None
+
+
+def _seen(ids: torch.Tensor, rows: int) -> torch.Tensor:
+    return (ids >= 0) & (ids < rows)
+
+
+def embed_tokens(table: torch.Tensor, ids: torch.Tensor,
+                 scale: float = 1.0) -> torch.Tensor:
+    """``scale * table[ids]``, [*ids.shape, D]."""
+    hip = _hip(table)
+    if hip is not None:
+        return hip.embedding_lookup(table, ids, scale)
+    seen = _seen(ids, table.shape[0])
+    out = table.new_zeros(*ids.shape, table.shape[1])
+    out[seen] = table[ids[seen].long()] * scale
+    return out
+
+
+def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
+               weights: Optional[torch.Tensor] = None,
+               scale: float = 1.0) -> torch.Tensor:
+    """``scale * sum_j weights[b, j] table[ids[b, j]]``, [B, D], of ids
+    [B, L]."""
+    hip = _hip(table)
+    if hip is not None:
+        return hip.embedding_bag(table, ids, None, weights, scale)
+    rows = embed_tokens(table, ids)
+    if weights is not None:
+        rows = rows * weights.unsqueeze(-1).to(rows.dtype)
+    return rows.sum(1) * scale
+
+
+def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
+                     weights: Optional[torch.Tensor] = None,
+                     scale: float = 1.0, out: Optional[torch.Tensor] = None
+                     ) -> torch.Tensor:
+    """``sum_tokens``'s gradient with respect to the table, [num_rows, D];
+    with ``out`` it is added to ``out``."""
+    hip = _hip(grad)
+    if hip is not None:
+        plan = hip.embedding_plan(ids, num_rows, pooled=True)
+        return hip.embedding_grad(grad, plan, weights, scale, out=out,
+                                  accumulate=out is not None)
+    g = grad.unsqueeze(1).expand(*ids.shape, grad.shape[1])
+    if weights is not None:
+        g = g * weights.unsqueeze(-1).to(g.dtype)
+    seen = _seen(ids, num_rows)
+    if out is None:
+        out = grad.new_zeros(num_rows, grad.shape[1])
+    return out.index_add_(0, ids[seen].long(), g[seen] * scale)
+
+
+def mean_weights(ids: torch.Tensor, num_rows: int) -> torch.Tensor:
+    """float32 [B, L]: one over the number of row b's words, so that the
+    weighted sum is their mean (zero for a row without any)."""
+    n = _seen(ids, num_rows).sum(1, keepdim=True).clamp(min=1)
+    return (1.0 / n.to(torch.float32)).expand(ids.shape).contiguous()
+
+
+class PadTokens(Transformer):
+    """Word ids of a document to one fixed length: cut off after it, filled
+    up with -1."""
+
+    def __init__(self, length: int):
+        if length < 1:
+            raise ValueError(f"PadTokens: expected a length of at least 1, "
+                             f"got {length}")
+        self.length = length
+
+    def apply(self, ids: Sequence[int]) -> torch.Tensor:
+        ids = list(ids)[:self.length]
+        return torch.tensor(ids + [-1] * (self.length - len(ids)),
+                            dtype=torch.int64)
+
+    def apply_dataset(self, ds: Dataset) -> TensorDataset:
+        rows = [self.apply(x) for x in ds.items()]
+        data = torch.stack(rows) if rows else \
+            torch.empty(0, self.length, dtype=torch.int64)
+        return TensorDataset(data.to(ds.runtime.device), ds.runtime)
+
+
+class _TableTransformer(BatchTransformer):
+    def __init__(self, table: torch.Tensor, scale: float = 1.0):
+        if table.dim() != 2 or not table.is_floating_point():
+            raise ValueError("expected a floating-point table [words, dim], "
+                             f"got {tuple(table.shape)} {table.dtype}")
+        self.table = table
+        self.scale = scale
+
+    def _resident(self, ids: torch.Tensor) -> torch.Tensor:
+        self.table = self.table.to(ids.device)
+        return self.table
+
+    @classmethod
+    def from_saved(cls, config, state):
+        return cls(state["table"], config["scale"])
+
+
+class TokenEmbedding(_TableTransformer):
+    """Word ids [..., L] to their rows of the table, scaled: [..., L, D]."""
+
+    def apply_batch(self, ids: torch.Tensor) -> torch.Tensor:
+        return embed_tokens(self._resident(ids), ids, self.scale)
+
+
+class MeanEmbedding(_TableTransformer):
+    """Word ids [n, L] to the mean of their rows of the table, scaled:
+    [n, D].  Unseen words (and PadTokens' filling) do not count."""
+
+    def apply_batch(self, ids: torch.Tensor) -> torch.Tensor:
+        table = self._resident(ids)
+        return sum_tokens(table, ids, mean_weights(ids, table.shape[0]),
+                          self.scale)

@@ -1,4 +1,5 @@
 from .cosine_features import CosineRandomFeatures
+from .dropout import dropout
 from .fft import PaddedFFT
 from .scaler import StandardScaler, StandardScalerModel
 from .misc import (ColumnSampler, LinearRectifier, NormalizeRows,
@@ -8,4 +9,5 @@ __all__ = [
     "CosineRandomFeatures", "PaddedFFT", "StandardScaler",
     "StandardScalerModel", "RandomSignNode", "LinearRectifier",
     "SignedHellingerMapper", "NormalizeRows", "ColumnSampler", "Sampler",
+    "dropout",
 ]

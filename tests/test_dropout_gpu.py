@@ -4,6 +4,8 @@ import numpy as np
 import pytest
 import torch
 
+from tests.philox import expected, philox
+
 pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -14,50 +16,6 @@ def hip():
     from keystone_amd import hip as h
     assert h.available(), "HIP extension must be built and loadable"
     return h
-
-
-def philox(counter, key):
-    """Philox4x32-10 on uint32 counters [n, 4] and a key of two words."""
-    c = [counter[:, i].astype(np.uint64) for i in range(4)]
-    k = [np.uint64(v) for v in key]
-    low, shift = np.uint64(0xffffffff), np.uint64(32)
-    for _ in range(10):
-        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
-        c = [(b >> shift) ^ c[1] ^ k[0], b & low,
-             (a >> shift) ^ c[3] ^ k[1], a & low]
-        k = [(k[0] + np.uint64(0x9E3779B9)) & low,
-             (k[1] + np.uint64(0xBB67AE85)) & low]
-    return np.stack(c, 1).astype(np.uint32)
-
-
-def test_philox_known_answers():
-    """The published vectors of the generator."""
-    cases = [((0, 0, 0, 0), (0, 0),
-              (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)),
-             ((0xffffffff,) * 4, (0xffffffff,) * 2,
-              (0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd)),
-             ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344),
-              (0xa4093822, 0x299f31d0),
-              (0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1))]
-    for c, k, want in cases:
-        got = philox(np.array([c], dtype=np.uint32), k)[0]
-        assert tuple(int(x) for x in got) == want
-
-
-def expected(x, p, seed, step):
-    n = x.numel()
-    b = np.arange(-(-n // 8), dtype=np.uint64)
-    low, shift = np.uint64(0xffffffff), np.uint64(32)
-    counter = np.stack([b & low, b >> shift,
-                        np.full_like(b, step & 0xffffffff),
-                        np.full_like(b, step >> 32)], 1)
-    words = philox(counter, (seed & 0xffffffff, seed >> 32))
-    bits = words.view(np.uint16).reshape(-1)[:n].astype(np.int64)
-    t = round(p * 65536)
-    keep = torch.from_numpy(bits >= t).view(x.shape)
-    scale = torch.tensor(65536 / (65536 - t), dtype=torch.float32)
-    y = x.cpu().float() * scale
-    return torch.where(keep, y, torch.zeros(())).to(x.dtype), keep
 
 
 @pytest.mark.parametrize("dtype", TYPES)
