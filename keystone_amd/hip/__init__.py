@@ -176,8 +176,8 @@ def _register_extra(lib: ctypes.CDLL) -> None:
         lib.ks_embedding_lookup.argtypes = [c_p, c_i, c_l, c_p, c_i, c_l, c_l,
                                             c_p, c_i, c_f, c_i, c_p]
         lib.ks_embedding_lookup.restype = c_i
-        lib.ks_segment_long.argtypes = []
-        lib.ks_segment_long.restype = c_i
+        lib.ks_segment_work.argtypes = [c_i, c_i, c_i]
+        lib.ks_segment_work.restype = c_l
         lib.ks_segment_sum.argtypes = [
             c_i, c_p, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_p, c_p, c_i,
             c_l, c_p, c_i, c_l, c_p, c_i, c_f, c_i, c_i, c_p]
@@ -229,8 +229,8 @@ def _stream() -> ctypes.c_void_p:
 
 
 def _raw_stream(device: torch.device) -> int:
-    """The current stream of ``device``."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device``, without making a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 _NO_GUARD = nullcontext()

@@ -72,8 +72,8 @@ def _pitch(t: torch.Tensor) -> int:
 
 def _width(D: int, *mats: torch.Tensor) -> int:
     """How many neighbours every row of every matrix can be read by at once."""
-    for v in (4, 2):
-        if D % v == 0 and all(
+    for v in (8, 4, 2):
+        if D % v == 0 and v * mats[0].element_size() <= 16 and all(
                 m.data_ptr() % (v * m.element_size()) == 0
                 and _pitch(m) % v == 0 for m in mats):
             return v
@@ -124,28 +124,18 @@ def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
     D = out.shape[1]
     if count == 0 or D == 0:
         return
-    part = None
-    if n > _long(lib):
-        chunks = -(-n // _long(lib))
-        part = torch.empty(chunks * 2 * ((D + 3) // 4 * 4),
-                           dtype=torch.float32, device=src.device)
+    vec = _width(D, src, out)
+    work = None
+    need = lib.ks_segment_work(n, D, vec)
+    if need:
+        work = torch.empty(need, dtype=torch.float32, device=src.device)
     with _guard(src.device):
         _check(lib.ks_segment_sum(
             kind, bounds, fixed, count, n, ids, ids_wide, V, order,
             _ptr(weights), keys, src.data_ptr(), _TYPES[src.dtype],
             _pitch(src), out.data_ptr(), _TYPES[out.dtype], _pitch(out),
-            _ptr(part), D, scale, int(accumulate), _width(D, src, out),
+            _ptr(work), D, scale, int(accumulate), vec,
             _raw_stream(src.device)), name)
-
-
-_long_entries = 0
-
-
-def _long(lib) -> int:
-    global _long_entries
-    if not _long_entries:
-        _long_entries = lib.ks_segment_long()
-    return _long_entries
 
 
 def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
@@ -223,8 +213,9 @@ def embedding_plan(ids: torch.Tensor, num_rows: int,
     rows = kept[2 * n:3 * n] if bagged else None
     starts = kept[-V - 1:]
     with _guard(ids.device):
-        work = torch.empty(lib.ks_token_sort_work(n, V), dtype=torch.int32,
-                           device=ids.device) if n else None
+        need = lib.ks_token_sort_work(n, V)
+        work = torch.empty(need, dtype=torch.int32, device=ids.device) \
+            if need else None
         _check(lib.ks_token_sort(
             ids.data_ptr(), int(ids.dtype == torch.int64), n, V, kind,
             _ptr(offsets), fixed, bags, keys.data_ptr(), order.data_ptr(),

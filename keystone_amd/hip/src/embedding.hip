@@ -82,13 +82,18 @@ __device__ __forceinline__ void bounds_of(const Segs& s, int i, int& b, int& e) 
     }
 }
 
-// The last segment that begins at or before entry i.
+// The last segment that begins at or before entry i, found by a whole wave:
+// each round splits what is left in 64.
 __device__ __forceinline__ int segment_of(const Segs& s, int i) {
     if (s.kind == 0) return i / s.fixed;
+    const int lane = threadIdx.x & 63;
     int lo = 0, hi = s.count;
     while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        if (bound_at(s, mid) <= i) lo = mid; else hi = mid;
+        const int step = (hi - lo + 63) / 64;
+        const long long at = (long long)lo + (long long)(lane + 1) * step;
+        const bool below = at < hi && bound_at(s, (int)at) <= i;
+        lo += __popcll(__ballot(below)) * step;
+        hi = min(hi, lo + step);
     }
     return lo;
 }
@@ -102,41 +107,120 @@ struct Entries {
     const int* keys;      // entry's segment, where it is known; else null
 };
 
+// Rows in flight a lane, and as many of the next entries' indices: an index
+// is on its way while the rows before it are.
+constexpr int U = 4;
+
+__device__ __forceinline__ void load_entries(const Entries& t, int i, int step,
+                                             int e, int (&row)[U],
+                                             float (&w)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = i + u * step;
+        row[u] = -1;
+        w[u] = 1.0f;
+        if (j < e) {
+            row[u] = row_of(t.ids, j);
+            if (t.weights) w[u] = t.weights[t.order ? t.order[j] : j];
+        }
+    }
+}
+
 // Sums src's rows of entries [b, e): lane (el, g) of a team takes every
-// `el_n`-th entry and the columns at `col`.  Four rows are in flight a lane.
+// `el_n`-th entry and the columns at `col`.
 template <typename TS, int VEC>
 __device__ __forceinline__ void add_entries(
         const Entries& t, const TS* src, long long ld, int col, bool live,
         int b, int e, int el, int el_n, float (&acc)[VEC]) {
-    constexpr int U = 4;
-    for (int i = b + el; i < e; i += U * el_n) {
-        int row[U];
-        float w[U];
+    using V = Vec<TS, VEC>;
+    int row[U];
+    float w[U];
+    int i = b + el;
+    if (i >= e) return;
+    load_entries(t, i, el_n, e, row, w);
+    do {
+        V v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = i + u * el_n;
-            row[u] = -1;
-            w[u] = 1.0f;
-            if (j < e) {
-                row[u] = row_of(t.ids, j);
-                if (t.weights) w[u] = t.weights[t.order ? t.order[j] : j];
-            }
-        }
-        float v[U][VEC];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (live && row[u] >= 0) {
-                load_row<TS, VEC>(src + (long long)row[u] * ld + col, v[u]);
-            } else {
+            v[u] = V{};
+            if (live && row[u] >= 0)
+                v[u] = *reinterpret_cast<const V*>(
+                    src + (long long)row[u] * ld + col);
+            else
                 w[u] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
-            }
         }
+        int next[U];
+        float wn[U];
+        i += U * el_n;
+        load_entries(t, i, el_n, e, next, wn);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] = fmaf(w[u], v[u][k], acc[k]);
+            for (int k = 0; k < VEC; ++k)
+                acc[k] = fmaf(w[u], (float)v[u][k], acc[k]);
+            row[u] = next[u];
+            w[u] = wn[u];
+        }
+    } while (i < e);
+}
+
+// The same with rows of eight lanes or more: each lane of a team finds one
+// entry's place and weight, and hands it to the others, so that an entry's
+// index work is done once and not by each lane of its row.  Places are counted
+// in VEC elements, in 32 bits.  The team is a part of a wave; `waves` of them
+// take turns.
+template <typename TS, int VEC>
+__device__ __forceinline__ void add_batches(
+        const Entries& t, const TS* src, unsigned pitch, int col, bool live,
+        int b, int e, int g_log, int el_log, int wave, int waves,
+        float (&acc)[VEC]) {
+    using V = Vec<TS, VEC>;
+    constexpr unsigned ABSENT = ~0u;
+    constexpr int R = 4;
+    const int t_n = 1 << (g_log + el_log), lane = threadIdx.x & 63;
+    const int own = lane & (t_n - 1), base = lane - own;
+    const int el = own >> g_log, el_n = 1 << el_log;
+    const V* const at = reinterpret_cast<const V*>(src) + col / VEC;
+    const auto find = [&](int j, unsigned& place, float& w) {
+        place = ABSENT;
+        w = 1.0f;
+        if (j < e) {
+            const int row = row_of(t.ids, j);
+            if (row >= 0) place = (unsigned)row * pitch;
+            if (t.weights) w = t.weights[t.order ? t.order[j] : j];
+        }
+    };
+    int i = b + wave * t_n;
+    unsigned place;
+    float w;
+    find(i + own, place, w);
+    for (; i < e; i += waves * t_n) {
+        unsigned next;
+        float wn;
+        find(i + waves * t_n + own, next, wn);
+        const int m = min(t_n, e - i);
+        for (int j = el; j - el < m; j += R * el_n) {
+            V v[R];
+            float f[R];
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int k = j + u * el_n;
+                const unsigned p = __shfl((int)place, base + (k & (t_n - 1)), 64);
+                f[u] = __shfl(w, base + (k & (t_n - 1)), 64);
+                v[u] = V{};
+                if (live && k < m && p != ABSENT)
+                    v[u] = at[p];
+                else
+                    f[u] = 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    acc[k] = fmaf(f[u], (float)v[u][k], acc[k]);
+        }
+        place = next;
+        w = wn;
     }
 }
 
@@ -155,124 +239,236 @@ __device__ __forceinline__ void put_row(TO* out, const float (&acc)[VEC],
     store_row<TO, VEC>(out, v);
 }
 
-// A segment over LONG entries is cut into chunks of LONG, each summed by a
-// wave of its own, and joined afterwards.
-constexpr int LONG = 128;
-
-// One team of g_n * el_n lanes a segment.
-template <typename TS, typename TO, int VEC>
-__global__ __launch_bounds__(256)
-void segment_sum_kernel(Segs segs, Entries t, const TS* __restrict__ src,
-                        long long ld, TO* __restrict__ out, long long ldo,
-                        int D, int g_log, int el_log, float scale,
-                        int accumulate) {
-    const int g_n = 1 << g_log, el_n = 1 << el_log;
-    const int lane = threadIdx.x;
-    const int g = lane & (g_n - 1), el = (lane >> g_log) & (el_n - 1);
-    const int team = lane >> (g_log + el_log), teams = 256 >> (g_log + el_log);
-    const int col = (blockIdx.y * g_n + g) * VEC;
-    const bool live = col < D;
-    for (long long s = (long long)blockIdx.x * teams + team; s < segs.count;
-         s += (long long)gridDim.x * teams) {
-        int b, e;
-        bounds_of(segs, (int)s, b, e);
-        if (e - b > LONG || (accumulate && e == b)) continue;
-        float acc[VEC] = {};
-        add_entries<TS, VEC>(t, src, ld, col, live, b, e, el, el_n, acc);
-        for (int m = g_n; m < g_n * el_n; m <<= 1)
+template <int VEC>
+__device__ __forceinline__ void add_lanes(float (&acc)[VEC], int from, int to) {
+    for (int m = from; m < to; m <<= 1)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], m, 64);
-        if (live && el == 0)
-            put_row<TO, VEC>(out + s * ldo + col, acc, scale, accumulate);
-    }
+        for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], m, 64);
 }
 
-// The segment that entry i lies in, if it is longer than LONG; else -1.
+// The sums of a block's four waves, each over its own lanes first, to its
+// first g_n threads.
+template <int VEC>
+__device__ __forceinline__ void add_block(float (&acc)[VEC], int g_n,
+                                          float (*red)[64 * VEC]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    add_lanes<VEC>(acc, g_n, 64);
+    __syncthreads();      // the sums before these have been read
+    if (wave && lane < g_n)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) red[wave - 1][k * 64 + lane] = acc[k];
+    __syncthreads();
+    if (threadIdx.x < g_n)
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] += red[w][k * 64 + lane];
+}
+
+// How a call's work is cut.  A row's columns lie on g_n lanes, el_n such
+// groups are a team and sum one segment; a block takes `strip` segments, in runs
+// of neighbours from all over: tokens by frequency have the long ones side by
+// side.  A segment over `cut` entries is summed by the whole block; one
+// over `chunk` is cut into chunks, each summed by a block of its own, and
+// joined by a second launch.
+struct Cut {
+    int g_log, el_log, strip, run_log;
+    int cut, chunk, chunks;
+    unsigned pitch;        // src's row pitch in VEC elements; 0: by add_entries
+    int by_entry;          // segments are looked for at entries, not by number
+    int dp;                // pitch of part
+    float* part;           // [chunks][2][dp]
+    int* begins;           // [chunks]: the long segment that begins there
+};
+
+template <typename TS, typename TO>
+struct Sum {
+    Segs segs;
+    Entries t;
+    const TS* src;
+    long long ld;
+    TO* out;
+    long long ldo;
+    int D;
+    float scale;
+    int accumulate;
+    Cut c;
+};
+
+// Sums entries [b, e) by the whole block.
+template <typename TS, typename TO, int VEC>
+__device__ __forceinline__ void add_by_block(const Sum<TS, TO>& a, int col,
+                                             bool live, int b, int e,
+                                             float (&acc)[VEC]) {
+    if (a.c.pitch)
+        add_batches<TS, VEC>(a.t, a.src, a.c.pitch, col, live, b, e, a.c.g_log,
+                             6 - a.c.g_log, threadIdx.x >> 6, 4, acc);
+    else
+        add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, b, e,
+                             threadIdx.x >> a.c.g_log, 256 >> a.c.g_log, acc);
+}
+
+// The long segment that entry i lies in, else -1; a whole wave's work.
 __device__ __forceinline__ int long_segment(const Segs& segs, const int* keys,
-                                            int i, int& b, int& e) {
+                                            int i, int chunk, int& b, int& e) {
     const int s = keys ? keys[i] : segment_of(segs, i);
     if (s >= segs.count) return -1;   // sorted tokens outside the table
     bounds_of(segs, s, b, e);
-    return (e - b > LONG && b <= i && i < e) ? s : -1;
+    return (e - b > chunk && b <= i && i < e) ? s : -1;
 }
 
-// Chunk c holds entries [c LONG, (c + 1) LONG).  Of the segments over LONG
-// at most one comes in from the left and at most one begins in it (and then
-// reaches its right end): two parts of part[c][2][dp].
-template <typename TS, int VEC>
-__global__ __launch_bounds__(256)
-void long_part_kernel(Segs segs, Entries t, const TS* __restrict__ src,
-                      long long ld, float* __restrict__ part, int dp, int D,
-                      int g_log, int chunks) {
-    const int c = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (c >= chunks) return;
-    const int g_n = 1 << g_log, el_n = 64 >> g_log;
-    const int g = lane & (g_n - 1), el = lane >> g_log;
+// Chunk c holds entries [c chunk, (c + 1) chunk).  Of the segments over
+// `chunk` at most one comes in from the left and at most one begins in it
+// (and then reaches its right end): two parts.
+template <typename TS, typename TO, int VEC>
+__device__ void sum_chunk(const Sum<TS, TO>& a, int c, float (*red)[64 * VEC]) {
+    __shared__ int found[2][3];
+    const int g_n = 1 << a.c.g_log, wave = threadIdx.x >> 6;
+    const int g = threadIdx.x & (g_n - 1);
     const int col = (blockIdx.y * g_n + g) * VEC;
-    const bool live = col < D;
-    const int i0 = c * LONG, i1 = min(segs.n, i0 + LONG);
+    const int i0 = c * a.c.chunk;
+    const int i1 = (int)min((long long)a.segs.n, (long long)i0 + a.c.chunk);
+    if (wave < 2) {
+        int b = 0, e = 0;
+        int s = long_segment(a.segs, a.t.keys, wave ? i1 - 1 : i0, a.c.chunk, b, e);
+        if ((b >= i0) != (wave == 1)) s = -1;
+        found[wave][0] = s;
+        found[wave][1] = max(b, i0);
+        found[wave][2] = min(e, i1);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.c.begins[c] = found[1][0];
 #pragma unroll 1
     for (int side = 0; side < 2; ++side) {
-        int b, e;
-        const int s = long_segment(segs, t.keys, side ? i1 - 1 : i0, b, e);
-        if (s < 0 || (b >= i0) != (side == 1)) continue;
+        if (found[side][0] < 0) continue;
         float acc[VEC] = {};
-        add_entries<TS, VEC>(t, src, ld, col, live, max(b, i0), min(e, i1),
-                             el, el_n, acc);
-        for (int m = g_n; m < 64; m <<= 1)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], m, 64);
-        if (live && el == 0)
-            store_row<float, VEC>(part + ((long long)c * 2 + side) * dp + col,
-                                  acc);
+        add_by_block<TS, TO, VEC>(a, col, col < a.D, found[side][1],
+                                  found[side][2], acc);
+        add_block<VEC>(acc, g_n, red);
+        if (threadIdx.x < g_n && col < a.D)
+            store_row<float, VEC>(
+                a.c.part + ((long long)c * 2 + side) * a.c.dp + col, acc);
     }
 }
 
-// Joins a long segment's parts: the block of the chunk that it begins in
-// adds them, every el_n-th by one row of threads, then the rows in LDS.
+template <typename TS, typename TO, int VEC>
+__global__ __launch_bounds__(256, 6)
+void segment_sum_kernel(Sum<TS, TO> a) {
+    __shared__ float red[3][64 * VEC];
+    // the strip's segments: number, first and last entry; those for a team
+    // from the front, those for the block from the back
+    __shared__ int seg[64], from[64], to[64], teams_share, blocks_share;
+    __shared__ unsigned long long empty;
+    if ((int)blockIdx.x < a.c.chunks) {
+        sum_chunk<TS, TO, VEC>(a, blockIdx.x, red);
+        return;
+    }
+    const int block = blockIdx.x - a.c.chunks, blocks = gridDim.x - a.c.chunks;
+    const int run = a.c.run_log;
+    const auto place = [=](int r) {
+        return (((long long)block + (long long)(r >> run) * blocks) << run) +
+               (r & ((1 << run) - 1));
+    };
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        long long s = place(lane);
+        bool mine = lane < a.c.strip;
+        if (a.c.by_entry) {
+            // the first entry of a token stands for it
+            const long long i = s;
+            mine = mine && i < a.segs.n &&
+                   (i == 0 || a.t.keys[i] != a.t.keys[i - 1]);
+            s = mine ? a.t.keys[i] : 0;
+        }
+        mine = mine && s < a.segs.count;
+        int b = 0, e = 0;
+        if (mine) bounds_of(a.segs, (int)s, b, e);
+        const bool some = mine && e > b && e - b <= a.c.chunk;
+        const bool one = some && e - b <= a.c.cut, all = some && !one;
+        const unsigned long long ones = __ballot(one), alls = __ballot(all);
+        const unsigned long long below = (1ull << lane) - 1;
+        if (some) {
+            const int at = one ? __popcll(ones & below)
+                               : 63 - __popcll(alls & below);
+            seg[at] = (int)s;
+            from[at] = b;
+            to[at] = e;
+        }
+        const unsigned long long none = __ballot(mine && e == b);
+        if (lane == 0) {
+            teams_share = __popcll(ones);
+            blocks_share = __popcll(alls);
+            empty = a.accumulate ? 0 : none;
+        }
+    }
+    __syncthreads();
+
+    const int g_n = 1 << a.c.g_log, el_n = 1 << a.c.el_log;
+    const int team_log = a.c.g_log + a.c.el_log;
+    const int g = threadIdx.x & (g_n - 1);
+    const int block_el = threadIdx.x >> a.c.g_log, block_el_n = 256 >> a.c.g_log;
+    const int el = block_el & (el_n - 1);
+    const int col = (blockIdx.y * g_n + g) * VEC;
+    const bool live = col < a.D;
+    if (empty && live) {
+        const float zero[VEC] = {};
+        for (int r = block_el; r < a.c.strip; r += block_el_n)
+            if (empty >> r & 1)
+                store_row<TO, VEC>(a.out + place(r) * a.ldo + col, zero);
+    }
+    for (int k = threadIdx.x >> team_log; k < teams_share; k += 256 >> team_log) {
+        float acc[VEC] = {};
+        if (a.c.pitch)
+            add_batches<TS, VEC>(a.t, a.src, a.c.pitch, col, live, from[k],
+                                 to[k], a.c.g_log, a.c.el_log, 0, 1, acc);
+        else
+            add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, from[k], to[k],
+                                 el, el_n, acc);
+        add_lanes<VEC>(acc, g_n, g_n * el_n);
+        if (live && el == 0)
+            put_row<TO, VEC>(a.out + (long long)seg[k] * a.ldo + col, acc,
+                             a.scale, a.accumulate);
+    }
+#pragma unroll 1
+    for (int k = 63; k > 63 - blocks_share; --k) {
+        float acc[VEC] = {};
+        add_by_block<TS, TO, VEC>(a, col, live, from[k], to[k], acc);
+        add_block<VEC>(acc, g_n, red);
+        if (live && threadIdx.x < g_n)
+            put_row<TO, VEC>(a.out + (long long)seg[k] * a.ldo + col, acc,
+                             a.scale, a.accumulate);
+    }
+}
+
+// Joins a long segment's parts: the block of the chunk that it begins in.
 template <typename TO, int VEC>
 __global__ __launch_bounds__(256)
-void long_join_kernel(Segs segs, const int* keys,
-                      const float* __restrict__ part, int dp,
-                      TO* __restrict__ out, long long ldo, int D, int g_log,
-                      float scale, int accumulate) {
-    __shared__ float red[256 * VEC];
-    const int c = blockIdx.x, i0 = c * LONG, i1 = min(segs.n, i0 + LONG);
+void segment_join_kernel(Segs segs, Cut c, TO* __restrict__ out, long long ldo,
+                         int D, float scale, int accumulate) {
+    __shared__ float red[3][64 * VEC];
+    const int s = c.begins[blockIdx.x];
+    if (s < 0) return;
     int b, e;
-    const int s = long_segment(segs, keys, i1 - 1, b, e);
-    if (s < 0 || b < i0) return;
-    const int last = (e - 1) / LONG;
-    const int g_n = 1 << g_log, el_n = 256 >> g_log;
-    const int g = threadIdx.x & (g_n - 1), el = threadIdx.x >> g_log;
+    bounds_of(segs, s, b, e);
+    const int last = (e - 1) / c.chunk;
+    const int g_n = 1 << c.g_log, el_n = 256 >> c.g_log;
+    const int g = threadIdx.x & (g_n - 1), el = threadIdx.x >> c.g_log;
     const int col = (blockIdx.y * g_n + g) * VEC;
-    const bool live = col < D;
     float acc[VEC] = {};
-    if (live) {
-        if (el == 0)
-            load_row<float, VEC>(part + ((long long)c * 2 + 1) * dp + col, acc);
+    if (col < D) {
+        const float* first = c.part + (long long)blockIdx.x * 2 * c.dp + col;
+        if (el == 0) load_row<float, VEC>(first + c.dp, acc);
 #pragma unroll 4
-        for (int k = c + 1 + el; k <= last; k += el_n) {
+        for (int k = 1 + el; k <= last - (int)blockIdx.x; k += el_n) {
             float v[VEC];
-            load_row<float, VEC>(part + (long long)k * 2 * dp + col, v);
+            load_row<float, VEC>(first + (long long)k * 2 * c.dp, v);
 #pragma unroll
             for (int q = 0; q < VEC; ++q) acc[q] += v[q];
         }
     }
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) red[q * 256 + threadIdx.x] = acc[q];
-    for (int half = el_n >> 1; half; half >>= 1) {
-        __syncthreads();
-        if (el < half)
-#pragma unroll
-            for (int q = 0; q < VEC; ++q)
-                red[q * 256 + threadIdx.x] +=
-                    red[q * 256 + threadIdx.x + half * g_n];
-    }
-    if (live && el == 0) {
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) acc[q] = red[q * 256 + threadIdx.x];
+    add_block<VEC>(acc, g_n, red);
+    if (col < D && threadIdx.x < g_n)
         put_row<TO, VEC>(out + (long long)s * ldo + col, acc, scale, accumulate);
-    }
 }
 
 // One team of g_n lanes a row, four rows in flight.
@@ -328,38 +524,80 @@ struct SumCall {
     long long ld;
     void* out;
     long long ldo;
-    float* part;
+    void* work;
     int D;
     float scale;
     int accumulate;
     hipStream_t stream;
 };
 
+// Lanes a row; entries a chunk: 32 a lane of the block, at most 512.
+// A row of 75 lanes is three times 32 of them rather than twice 64.
+int lanes_log(int D, int vec) {
+    const int cols = (D + vec - 1) / vec;
+    if (cols > 64 && (cols + 31) / 32 * 5 <= (cols + 63) / 64 * 8) return 5;
+    return log2_up(cols, 6);
+}
+int chunk_of(int D, int vec) {
+    const int c = 8192 >> lanes_log(D, vec);
+    return c < 512 ? c : 512;
+}
+
 template <typename TS, typename TO, int VEC>
-int segment_sum(const SumCall& c) {
-    const int cols = (c.D + VEC - 1) / VEC;
-    const int g_log = log2_up(cols, 6), slices = (cols + (1 << g_log) - 1) >> g_log;
-    // lanes that are left over share a segment's entries, up to one for each
-    // four that a segment has on average
-    const long long mean = c.segs.n / c.segs.count;
-    const int el_log = log2_up((int)(mean / 4 < 64 ? mean / 4 : 64), 6 - g_log);
-    const long long teams = 256 >> (g_log + el_log);
-    long long blocks = (c.segs.count + teams - 1) / teams;
-    if (blocks > (1 << 20)) blocks = 1 << 20;
-    const TS* src = (const TS*)c.src;
-    TO* out = (TO*)c.out;
+int segment_sum(const SumCall& a) {
+    const int cols = (a.D + VEC - 1) / VEC;
+    Cut c;
+    c.g_log = lanes_log(a.D, VEC);
+    const int slices = (cols + (1 << c.g_log) - 1) >> c.g_log;
+    c.chunk = chunk_of(a.D, VEC);
+    const long long span = a.t.ids.rows * (a.ld / VEC);
+    c.pitch = c.g_log >= 3 && span < 0xffffffffll ? (unsigned)(a.ld / VEC) : 0;
+    const bool some_long = a.segs.n > c.chunk &&
+                           !(a.segs.kind == 0 && a.segs.fixed <= c.chunk);
+    c.chunks = some_long ? (int)(((long long)a.segs.n + c.chunk - 1) / c.chunk) : 0;
+    c.dp = (a.D + 7) & ~7;
+    c.part = (float*)a.work;
+    c.begins = (int*)(c.part + (long long)c.chunks * 2 * c.dp);
+    c.by_entry = a.accumulate && a.t.keys && a.segs.n < a.segs.count;
+    const long long places = c.by_entry ? a.segs.n : a.segs.count;
+
+    // Lanes that are left over share a segment's entries, up to one for each
+    // four that a segment has on average.  Where waves of such teams do not
+    // fill the card, the whole block is a team.
+    const long long mean = a.segs.n / a.segs.count;
+    const int share = (int)(mean / 4 < 64 ? mean / 4 : 64);
+    c.el_log = log2_up(share, 6 - c.g_log);
+    const long long waves = (places << (c.g_log + c.el_log)) / 64;
+    const bool block_team = (share >> c.el_log) > 1 && waves < 8192;
+    // A block's segments: four times as many blocks as the card holds, to even
+    // out their lengths; where most segments are empty, one time.
+    long long strip = places / (mean ? 4096 : 1024) / 8 * 8;
+    strip = strip < 8 ? 8 : strip > 64 ? 64 : strip;
+    c.strip = block_team ? 1 : (int)strip;
+    // a run's rows are 64 bytes or more, to be written whole
+    c.run_log = 0;
+    while ((long long)a.D * sizeof(TO) << c.run_log < 64 &&
+           2 << c.run_log <= c.strip) ++c.run_log;
+    c.strip &= -1 << c.run_log;
+    // A segment stays with its team up to twice what a team sums on average
+    // on a full card (some 20 waves a compute unit), or four times the mean
+    // segment; a longer one would be the call's tail.
+    const long long full = 256 * 20 * 64 >> (c.g_log + c.el_log);
+    long long cut = 2 * (a.segs.n / full);
+    if (cut < 4 * mean) cut = 4 * mean;
+    if (cut < (2 * U) << c.el_log) cut = (2 * U) << c.el_log;
+    c.cut = (int)(cut < c.chunk ? cut : c.chunk);
+    if (block_team) c.cut = 0;
+
+    const long long blocks = c.chunks + (places + c.strip - 1) / c.strip;
+    const Sum<TS, TO> s{a.segs, a.t, (const TS*)a.src, a.ld, (TO*)a.out, a.ldo,
+                        a.D, a.scale, a.accumulate, c};
     segment_sum_kernel<TS, TO, VEC><<<dim3((unsigned)blocks, slices), 256, 0,
-        c.stream>>>(c.segs, c.t, src, c.ld, out, c.ldo, c.D, g_log, el_log,
-                    c.scale, c.accumulate);
-    if (c.segs.n > LONG && !(c.segs.kind == 0 && c.segs.fixed <= LONG)) {
-        const int chunks = (c.segs.n + LONG - 1) / LONG;
-        const int dp = (c.D + 3) & ~3;
-        long_part_kernel<TS, VEC><<<dim3((chunks + 3) / 4, slices), 256, 0,
-            c.stream>>>(c.segs, c.t, src, c.ld, c.part, dp, c.D, g_log, chunks);
-        long_join_kernel<TO, VEC><<<dim3(chunks, slices), 256, 0, c.stream>>>(
-            c.segs, c.t.keys, c.part, dp, out, c.ldo, c.D, g_log, c.scale,
-            c.accumulate);
-    }
+                                      a.stream>>>(s);
+    if (c.chunks)
+        segment_join_kernel<TO, VEC><<<dim3(c.chunks, slices), 256, 0,
+            a.stream>>>(a.segs, c, (TO*)a.out, a.ldo, a.D, a.scale,
+                        a.accumulate);
     return (int)hipGetLastError();
 }
 
@@ -368,7 +606,10 @@ int sum_by_width(const SumCall& c, int vec) {
     switch (vec) {
         case 1: return segment_sum<TS, TO, 1>(c);
         case 2: return segment_sum<TS, TO, 2>(c);
-        default: return segment_sum<TS, TO, 4>(c);
+        case 4: return segment_sum<TS, TO, 4>(c);
+        default:
+            if constexpr (sizeof(TS) == 2) return segment_sum<TS, TO, 8>(c);
+            return (int)hipErrorInvalidValue;
     }
 }
 
@@ -398,7 +639,11 @@ int lookup_by_width(const Ids& ids, long long n, const void* src, long long ld,
     switch (vec) {
         case 1: return lookup<T, 1>(ids, n, src, ld, out, D, scale, st);
         case 2: return lookup<T, 2>(ids, n, src, ld, out, D, scale, st);
-        default: return lookup<T, 4>(ids, n, src, ld, out, D, scale, st);
+        case 4: return lookup<T, 4>(ids, n, src, ld, out, D, scale, st);
+        default:
+            if constexpr (sizeof(T) == 2)
+                return lookup<T, 8>(ids, n, src, ld, out, D, scale, st);
+            return (int)hipErrorInvalidValue;
     }
 }
 
@@ -419,24 +664,28 @@ KS_EXPORT int ks_embedding_lookup(const void* ids, int ids_wide, long long n,
     }
 }
 
-KS_EXPORT int ks_segment_long() { return LONG; }
+// How many floats of workspace a segmented sum of n entries needs.
+KS_EXPORT long long ks_segment_work(int n, int D, int vec) {
+    const int chunk = chunk_of(D, vec);
+    if (n <= chunk) return 0;
+    return ((long long)n + chunk - 1) / chunk * (2 * ((D + 7) & ~7) + 1);
+}
 
 // out[count, D] (pitch ldo) = scale * sums of src's rows over segments.
 // kind/bounds/fixed: the segments; ids: each entry's row of src [V, D] (pitch
-// ld); order, weights, keys may be null.  part: two rows of ceil4(D) floats
-// for every ks_segment_long() entries; may be null for at most that many.
+// ld); order, weights, keys may be null.  work: ks_segment_work() floats.
 KS_EXPORT int ks_segment_sum(int kind, const void* bounds, int fixed,
                              int count, int n, const void* ids, int ids_wide,
                              long long V, const int* order,
                              const float* weights, const int* keys,
                              const void* src, int type, long long ld,
                              void* out, int out_type, long long ldo,
-                             float* part, int D, float scale, int accumulate,
+                             void* work, int D, float scale, int accumulate,
                              int vec, hipStream_t stream) {
     if (count == 0 || D == 0) return 0;
     const SumCall c{{bounds, kind, fixed, count, n},
                     {{ids, ids_wide, V}, order, weights, keys},
-                    src, ld, out, ldo, part, D, scale, accumulate, stream};
+                    src, ld, out, ldo, work, D, scale, accumulate, stream};
     switch (type) {
         case F32: return sum_by_out<float>(c, out_type, vec);
         case BF16: return sum_by_out<__bf16>(c, out_type, vec);
