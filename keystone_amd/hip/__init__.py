@@ -192,7 +192,7 @@ def _register_extra(lib: ctypes.CDLL) -> None:
         lib.ks_dropout.restype = c_i
         lib.ks_fp8_quantise.argtypes = [c_p, c_i, c_l, c_i, c_i, c_p, c_p, c_p]
         lib.ks_fp8_quantise.restype = c_i
-        lib.ks_fp8_splits.argtypes = [c_i, c_i, c_i]
+        lib.ks_fp8_splits.argtypes = [c_i, c_i, c_i, c_i]
         lib.ks_fp8_splits.restype = c_i
         lib.ks_fp8_gemm.argtypes = [c_p] * 6 + [c_i, c_p, c_i, c_i, c_i, c_p]
         lib.ks_fp8_gemm.restype = c_i

@@ -20,7 +20,8 @@ from . import _check, _guard, _load, _ptr, _raw_stream
 __all__ = ["Fp8Weight", "fp8_pack", "fp8_linear", "fp8_round"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_MAX = 2 ** 31 - 2048
+_MAX = 2 ** 31 - 2048      # rows
+_MAX_INNER = 2 ** 26
 
 
 class Fp8Weight:
@@ -84,9 +85,10 @@ def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
     if x.dtype not in _TYPES:
         raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, "
                            f"got {x.dtype}")
-    if x.dim() != 2 or max(x.shape) > _MAX:
-        raise ValueError(f"{name}: expected a matrix of at most {_MAX} a "
-                         f"side, got shape {tuple(x.shape)}")
+    if x.dim() != 2 or x.shape[0] > _MAX or x.shape[1] > _MAX_INNER:
+        raise ValueError(f"{name}: expected a matrix with at most "
+                         f"{_MAX_INNER} of the inner dimension and {_MAX} of "
+                         f"the other, got shape {tuple(x.shape)}")
     return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
 
 
@@ -159,7 +161,7 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
         return out.zero_() if bias is None else out.copy_(bias.expand(M, -1))
     with _guard(X.device):
         q, scales = _quantise(lib, X)
-        s = lib.ks_fp8_splits(M, W.N, K)
+        s = lib.ks_fp8_splits(_TYPES[X.dtype], M, W.N, K)
         part = torch.empty(s, M, W.N, dtype=torch.float32, device=X.device) \
             if s > 1 else None
         _check(lib.ks_fp8_gemm(

@@ -17,6 +17,7 @@
 #include "common.h"
 
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
@@ -226,6 +227,180 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
         }
 }
 
+// Large products with 16-bit results: a block of four waves has 256 x 256
+// outputs, a wave 128 x 128 of them in 256 accumulator registers, and runs
+// alone on its SIMD.  Per 128 of K and wave that is 64 matrix instructions of
+// 32 cycles.  W's chunks go to LDS (four stages of 32 KB, three steps ahead),
+// for both waves that need them; X's go straight to registers, each again as
+// soon as its last use is past, so that they have a whole step to arrive.
+// One barrier a step, in its middle: it ends the writing of the next stage
+// and the reading of the one before.
+constexpr int BIG = 256, STAGES = 4;
+
+// acc += w x^T with byte Q of the scales.  As inline assembly, for its place
+// among the loads: the compiler, to which the two are unrelated, gathers the
+// loads in front and runs out of registers.  Its result is next read as an
+// addend, 64 instructions on, or behind the kernel's own wait at the end.
+template <int Q>
+__device__ __forceinline__ void mfma_here(f32x4& acc, const i32x8& w,
+                                          const i32x8& x, unsigned ws,
+                                          unsigned xs) {
+    if constexpr (Q == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+                     "op_sel:[0,0,0] op_sel_hi:[0,0,0]"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
+    else if constexpr (Q == 1)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+                     "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
+    else if constexpr (Q == 2)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+                     "op_sel:[0,0,0] op_sel_hi:[1,1,0]"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+                     "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
+                     : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 1)
+void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
+                         const float* __restrict__ bias, int wide, int kper,
+                         int mblocks, int nblocks) {
+    __shared__ __attribute__((aligned(16))) unsigned char
+        stage[STAGES][BIG / 16 * CHUNK];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // neighbours along N share X's rows: let them share an L2
+    const unsigned id = ks_xcd_swizzle(blockIdx.x, gridDim.x);
+    const int bn = id % nblocks, bm = id / nblocks % mblocks;
+    const int split = id / nblocks / mblocks;
+    const int mtiles = ks_ceil_div(a.M, 16), ntiles = ks_ceil_div(a.N, 16);
+    const int m0 = bm * 16 + (wave >> 1) * 8, n0 = bn * 16 + (wave & 1) * 8;
+    const int k0 = split * kper, k1 = min(a.kblocks, k0 + kper);
+    const int kq = (a.kblocks + 3) / 4;
+
+    // tiles past the end are read as the last one, and their sums not kept
+    const unsigned char* xp[8];
+    const unsigned* xsp[8];
+    const unsigned* wsp[8];
+    __amdgpu_buffer_rsrc_t wp[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long t = min(m0 + i, mtiles - 1), u = min(n0 + i, ntiles - 1);
+        xp[i] = a.xq + t * a.kblocks * CHUNK;
+        xsp[i] = a.xs + t * kq * 16;
+        wsp[i] = a.ws + u * kq * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        wp[i] = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(a.wq + (long long)min(bn * 16 + wave * 4 + i, ntiles - 1) *
+                               a.kblocks * CHUNK),
+            0, a.kblocks * CHUNK, 0x00020000);
+    const auto fetch_w = [&](int kb) {
+        const int at = min(kb, k1 - 1) * CHUNK;
+        unsigned char* to = stage[kb % STAGES] + wave * 4 * CHUNK;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    wp[i],
+                    (__attribute__((address_space(3))) void*)(to + i * CHUNK + h * 1024),
+                    16, lane * 16, at + h * 1024, 0, 0);
+    };
+    const auto fetch_x = [&](int i, int kb) {
+        return load_chunk(xp[i] + (long long)min(kb, k1 - 1) * CHUNK, lane);
+    };
+    const auto read_w = [&](int j, int kb) {
+        return load_chunk(stage[kb % STAGES] + ((wave & 1) * 8 + j) * CHUNK, lane);
+    };
+
+    // scales of four blocks; those past this split's end are 2^-127 for both
+    // operands, whose products vanish
+    const int s = lane & 15;
+    const auto fetch_scales = [&](int kb, unsigned (&xs)[8], unsigned (&ws)[8]) {
+        const int at = min(kb / 4, kq - 1) * 16 + s;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xs[i] = xsp[i][at];
+            ws[i] = wsp[i][at];
+        }
+    };
+    const auto kept = [&](int kb) {
+        const int left = k1 - kb;
+        return left >= 4 ? ~0u : left <= 0 ? 0 : ~(~0u << 8 * left);
+    };
+
+    f32x4 acc[8][8] = {};
+    i32x8 x[8], w[8];
+    unsigned xs[8], ws[8], xn[8], wn[8];
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) fetch_w(k0 + k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fetch_x(i, k0);
+    fetch_scales(k0, xs, ws);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        xs[i] &= kept(k0);
+        ws[i] &= kept(k0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = read_w(j, k0);
+
+    const auto step = [&](auto q, int kb) {
+        fetch_w(kb + STAGES - 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                mfma_here<q.value>(acc[i][j], w[j], x[i], ws[j], xs[i]);
+                if (i == 7) w[j] = read_w(j, kb + 1);
+            }
+            x[i] = fetch_x(i, kb + 1);
+            if (i == 3) {
+                // what this wave put into stage kb + 1 has arrived: 56 loads
+                // or more were issued since
+                asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+        }
+    };
+    for (int kb = k0; kb < k1; kb += 4) {
+        fetch_scales(kb + 4, xn, wn);
+        step(std::integral_constant<int, 0>{}, kb);
+        step(std::integral_constant<int, 1>{}, kb + 1);
+        step(std::integral_constant<int, 2>{}, kb + 2);
+        step(std::integral_constant<int, 3>{}, kb + 3);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xs[i] = xn[i] & kept(kb + 4);
+            ws[i] = wn[i] & kept(kb + 4);
+        }
+    }
+    // the last matrix instructions have written their registers
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int m = (m0 + i) * 16 + (lane & 15);
+            const int n = (n0 + j) * 16 + (lane >> 4) * 4;
+            if (m >= a.M || n >= a.N) continue;
+            if (part)
+                store_columns<float>(part + (long long)split * a.M * a.N, a.N,
+                                     m, n, a.N, a.N % 4 == 0, acc[i][j], nullptr);
+            else
+                store_columns<T>(y, a.N, m, n, a.N, wide, acc[i][j], bias);
+        }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256)
 void fp8_join_kernel(const float* __restrict__ part, int splits, long long n,
@@ -250,8 +425,21 @@ int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
     return (int)hipGetLastError();
 }
 
-// How many ways K is split: enough waves to fill the card.
-int splits_of(int M, int N, int kblocks) {
+// Whether a product goes through the large kernel: enough outputs to fill half
+// its blocks.
+bool is_big(int type, int M, int N, int kblocks) {
+    return type != 0 && M >= 192 && N >= 192 && kblocks >= 16 &&
+           (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG) >= 32;
+}
+
+// How many ways K is split: enough blocks to fill the card.
+int splits_of(int type, int M, int N, int kblocks) {
+    if (is_big(type, M, N, kblocks)) {
+        const long long blocks = (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG);
+        long long s = 256 / blocks;
+        if (s > kblocks / 16) s = kblocks / 16;
+        return s < 1 ? 1 : (int)s;
+    }
     const long long blocks = (long long)ks_ceil_div(M, 64) * ks_ceil_div(N, 256);
     long long s = 512 / blocks;
     if (s > kblocks / 4) s = kblocks / 4;
@@ -259,13 +447,25 @@ int splits_of(int M, int N, int kblocks) {
 }
 
 template <typename T>
-int gemm(const Gemm& a, void* y, float* part, const float* bias, int splits,
+int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
          hipStream_t stream) {
+    const int splits = splits_of(type, a.M, a.N, a.kblocks);
     const int wide = a.N % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
-    const int kper = ks_ceil_div(a.kblocks, splits);
-    const dim3 grid(ks_ceil_div(a.N, 256), ks_ceil_div(a.M, 64), splits);
-    fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4><<<grid, 256, 0, stream>>>(
-        a, (T*)y, splits > 1 ? part : nullptr, bias, wide, kper);
+    // the large kernel's splits begin at whole words of scales
+    const int kper = ks_ceil_div(ks_ceil_div(a.kblocks, splits), 4) * 4;
+    float* parts = splits > 1 ? part : nullptr;
+    if constexpr (sizeof(T) == 2) {
+        if (is_big(type, a.M, a.N, a.kblocks)) {
+            const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
+            fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
+                a, (T*)y, parts, bias, wide, kper, mb, nb);
+        }
+    }
+    if (!is_big(type, a.M, a.N, a.kblocks)) {
+        const dim3 grid(ks_ceil_div(a.N, 256), ks_ceil_div(a.M, 64), splits);
+        fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4><<<grid, 256, 0, stream>>>(
+            a, (T*)y, parts, bias, wide, kper);
+    }
     if (splits > 1) {
         const long long n = (long long)a.M * a.N;
         long long blocks = (n + 255) / 256;
@@ -292,8 +492,8 @@ KS_EXPORT int ks_fp8_quantise(const void* x, int type, long long ld, int rows,
 }
 
 // How many [M, N] float32 parts ks_fp8_gemm needs; 1: none.
-KS_EXPORT int ks_fp8_splits(int M, int N, int K) {
-    return splits_of(M, N, ks_ceil_div(K, 128));
+KS_EXPORT int ks_fp8_splits(int type, int M, int N, int K) {
+    return splits_of(type, M, N, ks_ceil_div(K, 128));
 }
 
 KS_EXPORT int ks_fp8_gemm(const unsigned char* xq, const unsigned* xs,
@@ -302,10 +502,9 @@ KS_EXPORT int ks_fp8_gemm(const unsigned char* xq, const unsigned* xs,
                           int M, int K, int N, hipStream_t stream) {
     if (M == 0 || N == 0) return 0;
     const Gemm a{xq, xs, wq, ws, M, N, ks_ceil_div(K, 128)};
-    const int s = splits_of(M, N, a.kblocks);
     switch (type) {
-        case 0: return gemm<float>(a, y, part, bias, s, stream);
-        case 1: return gemm<__bf16>(a, y, part, bias, s, stream);
-        default: return gemm<_Float16>(a, y, part, bias, s, stream);
+        case 0: return gemm<float>(a, y, part, bias, type, stream);
+        case 1: return gemm<__bf16>(a, y, part, bias, type, stream);
+        default: return gemm<_Float16>(a, y, part, bias, type, stream);
     }
 }

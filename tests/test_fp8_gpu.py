@@ -45,8 +45,10 @@ def check(hip, got, X, W, b):
     if got.dtype != torch.float32:
         for k in range(0, X.shape[1], 128):
             a, c = x[:, k:k + 128].abs(), w[k:k + 128].abs()
-            tol += 128 * 2.0 ** -13 * torch.stack(
-                [(r[:, None] * c).amax(0) for r in a])
+            # (of many rows, the largest of each side: no less)
+            tol += 128 * 2.0 ** -13 * (torch.stack(
+                [(r[:, None] * c).amax(0) for r in a]) if len(a) <= 1024
+                else a.amax(1, keepdim=True) * c.amax(0))
     off = (got.cpu().double() - want).abs() - tol * (1 + 1e-9)
     assert off.max() <= 0, off.max()
 
@@ -105,6 +107,22 @@ def test_linear(hip, dtype, M, K, N):
         assert got.shape == (M, N) and got.dtype == dtype
         check(hip, got, X, W, bias)
     assert torch.equal(got, hip.fp8_linear(X, packed))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("M,K,N", [
+    (2100, 2176, 1030), (1500, 2049, 1600), (8192, 2560, 192),
+    (1025, 4224, 2050), (8200, 8192, 1000)])
+def test_large_product(hip, dtype, M, K, N):
+    """Blocks of 256 x 256, ragged on both sides; K of whole and of broken
+    fours of blocks, split and not."""
+    X, W, b = operands(M, K, N, dtype)
+    packed = hip.fp8_pack(W)
+    got = hip.fp8_linear(X, packed, b)
+    assert torch.equal(got, hip.fp8_linear(X, packed, b))
+    rows = torch.arange(0, M, 7)
+    rows = torch.cat([rows, torch.arange(M - 20, M)])
+    check(hip, got[rows.cuda()], X[rows.cuda()], W, b)
 
 
 def test_strided_and_misaligned_rows(hip):
