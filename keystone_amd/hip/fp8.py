@@ -160,8 +160,8 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
     if K == 0:
         return out.zero_() if bias is None else out.copy_(bias.expand(M, -1))
     with _guard(X.device):
-        q, scales = _quantise(lib, X)
         s = lib.ks_fp8_splits(_TYPES[X.dtype], M, W.N, K)
+        q, scales = _quantise(lib, X)
         part = torch.empty(s, M, W.N, dtype=torch.float32, device=X.device) \
             if s > 1 else None
         _check(lib.ks_fp8_gemm(

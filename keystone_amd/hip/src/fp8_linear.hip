@@ -44,26 +44,18 @@ __device__ __forceinline__ void load8(const T* p, bool wide, int left,
     }
 }
 
-// One wave a chunk: 16 rows by 128 of K.  scales[tile][K/512][16] has a
-// byte, 127 + e, for each of four blocks.
+// A lane's 32 elements of one block (row's pitch ld, K left from `k`): their
+// bytes, and 127 + the exponent.  The four lanes of a row, 16 apart, share it.
 template <typename T>
-__global__ __launch_bounds__(256)
-void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
-                         int K, int tiles, int kblocks, int wide,
-                         unsigned char* __restrict__ q,
-                         unsigned char* __restrict__ scales) {
-    const long long chunk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (chunk >= (long long)tiles * kblocks) return;
-    const int kb = (int)(chunk % kblocks), tile = (int)(chunk / kblocks);
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    const int row = tile * 16 + (lane & 15);
+__device__ __forceinline__ int quantise_block(const T* row, int k, int K, int g,
+                                              bool live, bool wide,
+                                              uint32_t (&w)[8]) {
     float v[4][8];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int k = kb * 128 + j * 32 + g * 8;
-        load8(x + (long long)row * ld + k, wide && row < rows,
-              row < rows ? K - k : 0, v[j]);
+        const int at = k + j * 32 + g * 8;
+        load8(row + at, wide && live, live ? K - at : 0, v[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
@@ -76,7 +68,6 @@ void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
     if (top == 0 || bad) e = 0;
     if (e < -117) e = -117;
     const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-    uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -90,12 +81,31 @@ void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
             w[2 * j + h] = bad ? 0x7f7f7f7fu : (uint32_t)d;
         }
     }
+    return 127 + e;
+}
+
+// One wave a chunk: 16 rows by 128 of K.  scales[tile][K/512][16] has a
+// byte, 127 + e, for each of four blocks.
+template <typename T>
+__global__ __launch_bounds__(256)
+void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
+                         int K, int tiles, int kblocks, int wide,
+                         unsigned char* __restrict__ q,
+                         unsigned char* __restrict__ scales) {
+    const long long chunk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (chunk >= (long long)tiles * kblocks) return;
+    const int kb = (int)(chunk % kblocks), tile = (int)(chunk / kblocks);
+    const int lane = threadIdx.x & 63;
+    const int row = tile * 16 + (lane & 15);
+    uint32_t w[8];
+    const int e = quantise_block(x + (long long)row * ld, kb * 128, K, lane >> 4,
+                                 row < rows, wide, w);
     unsigned char* to = q + chunk * CHUNK + lane * 16;
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(to + 1024) = make_uint4(w[4], w[5], w[6], w[7]);
     if (lane < 16)
         scales[((long long)tile * ((kblocks + 3) / 4) + kb / 4) * 64 +
-               lane * 4 + (kb & 3)] = (unsigned char)(127 + e);
+               lane * 4 + (kb & 3)] = (unsigned char)e;
 }
 
 struct Gemm {
@@ -133,13 +143,18 @@ __device__ __forceinline__ f32x4 mfma(i32x8 w, i32x8 x, f32x4 acc, int ws,
         w, x, acc, 0, 0, 0, ws, 0, xs);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
-                                              int N, bool wide, f32x4 v,
-                                              const float* bias) {
+// Four columns' bias; none past N.
+__device__ __forceinline__ f32x4 bias_at(const float* bias, int n, int N) {
+    f32x4 v = {};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (bias && n + k < N) v[k] += bias[n + k];
+        if (bias && n + k < N) v[k] = bias[n + k];
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
+                                              int N, bool wide, f32x4 v) {
     T* to = y + m * ld + n;
     if (wide && n + 4 <= N) {
         using V4 = T __attribute__((ext_vector_type(4)));
@@ -154,8 +169,71 @@ __device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
     }
 }
 
+// A wave's tiles: column n + 16 j, row m + 16 i of y, or of `part` in 32 bits.
+template <typename T, int TM, int TN>
+__device__ __forceinline__ void store_tiles(const f32x4 (&acc)[TM][TN], T* y,
+                                            float* part, const float* bias,
+                                            int m, int n, int M, int N,
+                                            bool wide) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int at = n + j * 16;
+        if (at >= N) continue;
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                if (m + i * 16 < M)
+                    store_columns<float>(part, N, m + i * 16, at, N, N % 4 == 0,
+                                         acc[i][j]);
+        } else {
+            const f32x4 b = bias_at(bias, at, N);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                if (m + i * 16 < M)
+                    store_columns<T>(y, N, m + i * 16, at, N, wide, acc[i][j] + b);
+        }
+    }
+}
+
+// acc += w x^T over 128 of K, for either kind of output.
+template <bool EXACT, int TM, int TN>
+__device__ __forceinline__ void multiply(const i32x8 (&xf)[TM], const int (&xs)[TM],
+                                         const i32x8 (&wf)[TN], const int (&ws)[TN],
+                                         f32x4 (&acc)[TM][TN]) {
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            bf16x8 x[TM], w[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                x[i] = widen(xf[i][2 * s], xf[i][2 * s + 1], xs[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                w[j] = widen(wf[j][2 * s], wf[j][2 * s + 1], ws[j]);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        w[j], x[i], acc[i][j], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = mfma(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
+    }
+}
+
+__device__ __forceinline__ int scale_at(const unsigned* scales, int kq, int tile,
+                                        int kb, int lane) {
+    return (int)(scales[((long long)tile * kq + kb / 4) * 16 + (lane & 15)]
+                 >> (8 * (kb & 3))) & 255;
+}
+
 // A wave has TM x TN tiles of 16 x 16; its operands come straight from
-// memory.  Split s of gridDim.z takes K blocks [s kper, (s + 1) kper); with
+// memory.  Waves are counted along N first: neighbours share X's rows.  Split s of gridDim.y takes K blocks [s kper, (s + 1) kper); with
 // more than one split, `part` [splits][M][N] takes the sums.
 // EXACT: products and sums for 32-bit outputs.
 template <typename T, int TM, int TN, bool EXACT>
@@ -164,9 +242,11 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
                      const float* __restrict__ bias, int wide, int kper) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int mtiles = ks_ceil_div(a.M, 16), ntiles = ks_ceil_div(a.N, 16);
-    const int m0 = blockIdx.y * TM, n0 = (blockIdx.x * 4 + wave) * TN;
-    if (n0 >= ntiles) return;
-    const int k0 = blockIdx.z * kper, k1 = min(a.kblocks, k0 + kper);
+    const int groups = ks_ceil_div(ntiles, TN);
+    const int id = blockIdx.x * 4 + wave;
+    const int m0 = id / groups * TM, n0 = id % groups * TN;
+    if (m0 >= mtiles) return;
+    const int k0 = blockIdx.y * kper, k1 = min(a.kblocks, k0 + kper);
     const int kq = (a.kblocks + 3) / 4;
     f32x4 acc[TM][TN] = {};
     for (int kb = k0; kb < k1; ++kb) {
@@ -176,55 +256,64 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
         for (int i = 0; i < TM; ++i) {
             const int t = min(m0 + i, mtiles - 1);
             xf[i] = load_chunk(a.xq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
-            xs[i] = (int)(a.xs[((long long)t * kq + kb / 4) * 16 + (lane & 15)]
-                          >> (8 * (kb & 3))) & 255;
+            xs[i] = scale_at(a.xs, kq, t, kb, lane);
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int t = min(n0 + j, ntiles - 1);
             wf[j] = load_chunk(a.wq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
-            ws[j] = (int)(a.ws[((long long)t * kq + kb / 4) * 16 + (lane & 15)]
-                          >> (8 * (kb & 3))) & 255;
+            ws[j] = scale_at(a.ws, kq, t, kb, lane);
         }
-        if constexpr (EXACT) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                bf16x8 x[TM], w[TN];
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-                    x[i] = widen(xf[i][2 * s], xf[i][2 * s + 1], xs[i]);
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    w[j] = widen(wf[j][2 * s], wf[j][2 * s + 1], ws[j]);
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            w[j], x[i], acc[i][j], 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    acc[i][j] = mfma(wf[j], xf[i], acc[i][j], ws[j], xs[i]);
-        }
+        multiply<EXACT, TM, TN>(xf, xs, wf, ws, acc);
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
+    store_tiles<T, TM, TN>(
+        acc, y, part ? part + (long long)blockIdx.y * a.M * a.N : nullptr, bias,
+        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N, wide);
+}
+
+// Few rows, or few columns: a block has one tile of 16 rows by TN of 16
+// columns, its 16 waves share K (of split blockIdx.y) and add up in LDS.
+template <typename T, int TN>
+__global__ __launch_bounds__(1024)
+void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
+                     const float* __restrict__ bias, int wide, int kper) {
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ f32x4 sums[16][TN][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int ntiles = ks_ceil_div(a.N, 16), groups = ks_ceil_div(ntiles, TN);
+    const int tile = blockIdx.x / groups, n0 = blockIdx.x % groups * TN;
+    const int kq = (a.kblocks + 3) / 4;
+    const int k1 = min(a.kblocks, ((int)blockIdx.y + 1) * kper);
+    f32x4 acc[1][TN] = {};
+    for (int kb = blockIdx.y * kper + wave; kb < k1; kb += 16) {
+        i32x8 xf[1], wf[TN];
+        int xs[1], ws[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int m = (m0 + i) * 16 + (lane & 15);
-            const int n = (n0 + j) * 16 + (lane >> 4) * 4;
-            if (m >= a.M || n >= a.N) continue;
-            if (part)
-                store_columns<float>(part + (long long)blockIdx.z * a.M * a.N,
-                                     a.N, m, n, a.N, a.N % 4 == 0, acc[i][j],
-                                     nullptr);
-            else
-                store_columns<T>(y, a.N, m, n, a.N, wide, acc[i][j], bias);
+            const int t = min(n0 + j, ntiles - 1);
+            wf[j] = load_chunk(a.wq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
+            ws[j] = scale_at(a.ws, kq, t, kb, lane);
         }
+        xf[0] = load_chunk(a.xq + ((long long)tile * a.kblocks + kb) * CHUNK, lane);
+        xs[0] = scale_at(a.xs, kq, tile, kb, lane);
+        multiply<EXACT, 1, TN>(xf, xs, wf, ws, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[0][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TN * 64; i += 1024) {
+        const int j = i >> 6, l = i & 63;
+        f32x4 s = sums[0][j][l];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += sums[w][j][l];
+        const int m = tile * 16 + (l & 15), n = (n0 + j) * 16 + (l >> 4) * 4;
+        if (m >= a.M || n >= a.N) continue;
+        if (part)
+            store_columns<float>(part + (long long)blockIdx.y * a.M * a.N, a.N,
+                                 m, n, a.N, a.N % 4 == 0, s);
+        else
+            store_columns<T>(y, a.N, m, n, a.N, wide, s + bias_at(bias, n, a.N));
+    }
 }
 
 // Large products with 16-bit results: a block of four waves has 256 x 256
@@ -386,19 +475,9 @@ void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
     }
     // the last matrix instructions have written their registers
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int m = (m0 + i) * 16 + (lane & 15);
-            const int n = (n0 + j) * 16 + (lane >> 4) * 4;
-            if (m >= a.M || n >= a.N) continue;
-            if (part)
-                store_columns<float>(part + (long long)split * a.M * a.N, a.N,
-                                     m, n, a.N, a.N % 4 == 0, acc[i][j], nullptr);
-            else
-                store_columns<T>(y, a.N, m, n, a.N, wide, acc[i][j], bias);
-        }
+    store_tiles<T, 8, 8>(
+        acc, y, part ? part + (long long)split * a.M * a.N : nullptr, bias,
+        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N, wide);
 }
 
 template <typename T>
@@ -425,45 +504,91 @@ int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
     return (int)hipGetLastError();
 }
 
-// Whether a product goes through the large kernel: enough outputs to fill half
-// its blocks.
-bool is_big(int type, int M, int N, int kblocks) {
-    return type != 0 && M >= 192 && N >= 192 && kblocks >= 16 &&
-           (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG) >= 32;
+// Which kernel a product goes through.
+enum Kind { ROWS, TILES, LARGE };
+
+Kind kind_of(int type, int M, int N, int kblocks) {
+    const int mt = ks_ceil_div(M, 16), nt = ks_ceil_div(N, 16);
+    if (mt == 1 || (long long)mt * nt <= 512 || (mt <= 64 && nt <= 16))
+        return ROWS;
+    // at least four steps for each compute unit.  2048 x 2048 x 2048 bf16 has
+    // four: 37 us against 38 us by TILES; 8192 x 1024 x 2000 eight: 39 against
+    // 53; 512 x 65536 x 1000 sixteen: 59 against 87; 1024 x 4096 x 1000 two:
+    // 38 against 28
+    if (type != 0 && M >= 192 && N >= 192 && kblocks >= 8 &&
+        (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG) * kblocks >= 1024)
+        return LARGE;
+    return TILES;
+}
+
+// A wave's tiles of rows in fp8_gemm_kernel: two where four would leave the
+// card short of waves.  1000 x 1000 x 1000 f16: 13.5 us with two, 17.8 us with
+// four; 8192 x 8192 x 1000 f32: 181 us and 175 us.
+int tiles_down(int M, int N) {
+    return (long long)ks_ceil_div(M, 64) * ks_ceil_div(N, 64) < 1024 ? 2 : 4;
 }
 
 // How many ways K is split: enough blocks to fill the card.
 int splits_of(int type, int M, int N, int kblocks) {
-    if (is_big(type, M, N, kblocks)) {
+    const Kind kind = kind_of(type, M, N, kblocks);
+    if (kind == ROWS) {
+        // 65 MB of W take 27 us from 63 blocks, and 17 us from 252 and a join;
+        // 16 MB take 7.4 us and gain nothing
+        long long s = 256 / ((long long)ks_ceil_div(M, 16) * ks_ceil_div(N, 16));
+        if (s > kblocks / 128) s = kblocks / 128;
+        return s < 1 || kblocks < 256 ? 1 : (int)s;
+    }
+    if (kind == LARGE) {
         const long long blocks = (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG);
         long long s = 256 / blocks;
-        if (s > kblocks / 16) s = kblocks / 16;
+        if (s > kblocks / 8) s = kblocks / 8;
         return s < 1 ? 1 : (int)s;
     }
-    const long long blocks = (long long)ks_ceil_div(M, 64) * ks_ceil_div(N, 256);
-    long long s = 512 / blocks;
+    const long long waves = (long long)ks_ceil_div(M, 16 * tiles_down(M, N)) *
+                            ks_ceil_div(N, 64);
+    long long s = 2048 / waves;
     if (s > kblocks / 4) s = kblocks / 4;
     return s < 1 ? 1 : (int)s;
 }
 
 template <typename T>
+void rows(const Gemm& a, T* y, float* part, const float* bias, int wide,
+          int splits, int kper, hipStream_t stream) {
+    const int nt = ks_ceil_div(a.N, 16), mt = ks_ceil_div(a.M, 16);
+    // 1021 x 8192 x 147: 12 us with three columns of tiles a block in 32 bits
+    // (15 with five, whose widening takes longer), with five in 16 (13 with
+    // three)
+    constexpr int WIDE = sizeof(T) == 4 ? 3 : 5;
+    const int tn = (long long)mt * nt <= 512 ? 1 : WIDE;
+    const unsigned grid = (unsigned)mt * ks_ceil_div(nt, tn);
+    auto* kernel = tn == 1 ? fp8_rows_kernel<T, 1> : fp8_rows_kernel<T, WIDE>;
+    kernel<<<dim3(grid, splits), 1024, 0, stream>>>(a, y, part, bias, wide, kper);
+}
+
+template <typename T>
 int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
          hipStream_t stream) {
+    const Kind kind = kind_of(type, a.M, a.N, a.kblocks);
     const int splits = splits_of(type, a.M, a.N, a.kblocks);
     const int wide = a.N % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
-    // the large kernel's splits begin at whole words of scales
+    // splits begin at whole words of scales
     const int kper = ks_ceil_div(ks_ceil_div(a.kblocks, splits), 4) * 4;
     float* parts = splits > 1 ? part : nullptr;
-    if constexpr (sizeof(T) == 2) {
-        if (is_big(type, a.M, a.N, a.kblocks)) {
+    if (kind == ROWS) {
+        rows<T>(a, (T*)y, parts, bias, wide, splits, kper, stream);
+    } else if (kind == LARGE) {
+        if constexpr (sizeof(T) == 2) {
             const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
             fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
                 a, (T*)y, parts, bias, wide, kper, mb, nb);
         }
-    }
-    if (!is_big(type, a.M, a.N, a.kblocks)) {
-        const dim3 grid(ks_ceil_div(a.N, 256), ks_ceil_div(a.M, 64), splits);
-        fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4><<<grid, 256, 0, stream>>>(
+    } else {
+        const int down = tiles_down(a.M, a.N);
+        const long long waves = (long long)ks_ceil_div(a.N, 64) *
+                                ks_ceil_div(a.M, 16 * down);
+        auto* kernel = down == 2 ? fp8_gemm_kernel<T, 2, 4, sizeof(T) == 4>
+                                 : fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4>;
+        kernel<<<dim3((unsigned)((waves + 3) / 4), splits), 256, 0, stream>>>(
             a, (T*)y, parts, bias, wide, kper);
     }
     if (splits > 1) {
@@ -496,6 +621,8 @@ KS_EXPORT int ks_fp8_splits(int type, int M, int N, int K) {
     return splits_of(type, M, N, ks_ceil_div(K, 128));
 }
 
+// y [M, N] = X W + bias of quantised operands; y's type as above, bias may be
+// null.
 KS_EXPORT int ks_fp8_gemm(const unsigned char* xq, const unsigned* xs,
                           const unsigned char* wq, const unsigned* ws,
                           const float* bias, void* y, int type, float* part,
