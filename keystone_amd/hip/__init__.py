@@ -32,7 +32,6 @@ import subprocess
 import sys
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
-from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -228,19 +227,19 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _raw_stream(device: torch.device) -> int:
-    """The current stream of ``device``, without making a Stream object."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-_NO_GUARD = nullcontext()
-
-
-def _guard(device: torch.device):
-    """Makes ``device`` current for a launch, where it is not."""
-    if device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+def _launch(name: str, device: torch.device, *args) -> None:
+    """Calls the library's ``name`` on ``device``, made current where it is
+    not, and on its current stream, which goes last."""
+    fn = getattr(_lib, name)
+    at = device.index
+    if at == torch.cuda.current_device():
+        # the handle alone: a Stream object costs more than the launch
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(at):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    if code != 0:
+        _check(code, name)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

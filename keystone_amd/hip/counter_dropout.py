@@ -6,7 +6,7 @@ from typing import Optional, Union
 
 import torch
 
-from . import _check, _guard, _load, _ptr, _raw_stream
+from . import _launch, _load, _ptr
 
 __all__ = ["dropout", "dropout_threshold"]
 
@@ -33,7 +33,7 @@ def dropout(x: torch.Tensor, p: float, seed: int,
     ``step``: a number below 2^64, or an int64 tensor of one element on x's
     device, which a captured graph reads at each replay.  ``out`` may be
     ``x``."""
-    lib = _load()
+    _load()
     if not x.is_cuda:
         raise RuntimeError("dropout.x: expected CUDA tensor")
     if x.dtype not in _TYPES:
@@ -64,9 +64,6 @@ def dropout(x: torch.Tensor, p: float, seed: int,
         lo, size = out.data_ptr(), x.numel() * x.element_size()
         if 0 < abs(x.data_ptr() - lo) < size:
             raise ValueError("dropout: out overlaps x")
-    with _guard(x.device):
-        _check(lib.ks_dropout(x.data_ptr(), out.data_ptr(), x.numel(),
-                              _TYPES[x.dtype], t, 65536 / (65536 - t), seed,
-                              step, _ptr(at), _raw_stream(x.device)),
-               "ks_dropout")
+    _launch("ks_dropout", x.device, x.data_ptr(), out.data_ptr(), x.numel(),
+            _TYPES[x.dtype], t, 65536 / (65536 - t), seed, step, _ptr(at))
     return out

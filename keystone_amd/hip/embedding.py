@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from . import _check, _guard, _load, _ptr, _raw_stream
+from . import _launch, _load, _ptr
 
 __all__ = ["EmbeddingPlan", "embedding_lookup", "embedding_bag",
            "embedding_plan", "embedding_grad"]
@@ -39,9 +39,10 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dim() != 2:
         raise ValueError(f"{name}: expected a matrix, got shape "
                          f"{tuple(t.shape)}")
-    if t.shape[0] > _MAX or t.shape[1] > _MAX:
+    rows, D = t.shape
+    if rows > _MAX or D > _MAX:
         raise ValueError(f"{name}: {tuple(t.shape)} is over {_MAX} a side")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if D > 1 and t.stride(1) != 1:
         return t.contiguous()
     return t
 
@@ -70,14 +71,11 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _width(D: int, *mats: torch.Tensor) -> int:
-    """How many neighbours every row of every matrix can be read by at once."""
-    for v in (8, 4, 2):
-        if D % v == 0 and v * mats[0].element_size() <= 16 and all(
-                m.data_ptr() % (v * m.element_size()) == 0
-                and _pitch(m) % v == 0 for m in mats):
-            return v
-    return 1
+def _width(D: int, size: int, pitch: int, address: int) -> int:
+    """How many neighbours every row of a matrix can be read by at once: a
+    power of two, 16 bytes at most."""
+    x = (D | pitch) * size | address | 16
+    return max((x & -x) // size, 1)
 
 
 def _bags(ids: torch.Tensor, offsets: Optional[torch.Tensor], name: str):
@@ -109,33 +107,39 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     n = ids.numel()
     if n and D:
-        flat = out.view(n, D)
-        with _guard(table.device):
-            _check(lib.ks_embedding_lookup(
-                ids.data_ptr(), int(ids.dtype == torch.int64), n,
-                table.data_ptr(), _TYPES[table.dtype], V, _pitch(table),
-                flat.data_ptr(), D, scale, _width(D, table, flat),
-                _raw_stream(table.device)), "ks_embedding_lookup")
+        size = table.element_size()
+        pitch = table.stride(0) if V > 1 else D
+        address = table.data_ptr()
+        _launch("ks_embedding_lookup", table.device, ids.data_ptr(),
+                ids.dtype == torch.int64, n, address, _TYPES[table.dtype], V,
+                pitch, out.data_ptr(), D, scale,
+                _width(D, size, pitch, address))
     return out
 
 
 def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
-                 weights, keys, src, out, scale, accumulate, name):
+                 weights, keys, src, out, scale, accumulate):
+    name = "ks_segment_sum"
     D = out.shape[1]
     if count == 0 or D == 0:
         return
-    vec = _width(D, src, out)
+    pitch, out_pitch = _pitch(src), _pitch(out)
+    at, to = src.data_ptr(), out.data_ptr()
+    size, out_size = src.element_size(), out.element_size()
+    # as many as a row of src is read by; out's rows are then written by one
+    # or two stores
+    vec = _width(D, size, pitch, at)
+    x = out_pitch * out_size | to
+    while vec > 1 and x % (vec * out_size):
+        vec //= 2
     work = None
     need = lib.ks_segment_work(n, D, vec)
     if need:
         work = torch.empty(need, dtype=torch.float32, device=src.device)
-    with _guard(src.device):
-        _check(lib.ks_segment_sum(
-            kind, bounds, fixed, count, n, ids, ids_wide, V, order,
-            _ptr(weights), keys, src.data_ptr(), _TYPES[src.dtype],
-            _pitch(src), out.data_ptr(), _TYPES[out.dtype], _pitch(out),
-            _ptr(work), D, scale, int(accumulate), vec,
-            _raw_stream(src.device)), name)
+    _launch(name, src.device, kind, bounds, fixed, count, n, ids, ids_wide, V,
+            order, _ptr(weights), keys, at, _TYPES[src.dtype], pitch, to,
+            _TYPES[out.dtype], out_pitch, _ptr(work), D, scale, accumulate,
+            vec)
 
 
 def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
@@ -164,8 +168,8 @@ def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
         return torch.zeros(bags, D, dtype=table.dtype, device=table.device)
     out = torch.empty(bags, D, dtype=table.dtype, device=table.device)
     _segment_sum(lib, kind, _ptr(offsets), fixed, bags, n, ids.data_ptr(),
-                 int(ids.dtype == torch.int64), V, None, weights, None, table,
-                 out, scale, False, "embedding_bag")
+                 ids.dtype == torch.int64, V, None, weights, None, table, out,
+                 scale, False)
     return out
 
 
@@ -179,11 +183,33 @@ class EmbeddingPlan:
     bags (positions themselves where the ids are not pooled); ``keys`` [n]:
     their tokens; ``starts`` [V + 1]: where each token begins."""
 
-    def __init__(self, num_rows, num_bags, n, order, rows, keys, starts):
+    def __init__(self, kept: torch.Tensor, num_rows: int, num_bags: int,
+                 n: int, bagged: bool):
         self.num_rows, self.num_bags, self.n = num_rows, num_bags, n
-        self.order, self.rows = order, rows
-        self.keys, self.starts = keys, starts
-        self.device = starts.device
+        self.device = kept.device
+        # keys, order, rows where there are bags, starts: one allocation
+        self._kept, self._bagged = kept, bagged
+        self._keys = kept.data_ptr()
+        self._order = self._keys + 4 * n
+        self._rows = self._order + (4 * n if bagged else 0)
+        self._starts = self._rows + 4 * n
+
+    @property
+    def keys(self) -> torch.Tensor:
+        return self._kept[:self.n]
+
+    @property
+    def order(self) -> torch.Tensor:
+        return self._kept[self.n:2 * self.n]
+
+    @property
+    def rows(self) -> torch.Tensor:
+        return self._kept[2 * self.n:3 * self.n] if self._bagged \
+            else self.order
+
+    @property
+    def starts(self) -> torch.Tensor:
+        return self._kept[self._kept.numel() - self.num_rows - 1:]
 
 
 def embedding_plan(ids: torch.Tensor, num_rows: int,
@@ -209,20 +235,15 @@ def embedding_plan(ids: torch.Tensor, num_rows: int,
                          f"rows are over {_MAX}")
     kept = torch.empty((3 if bagged else 2) * n + V + 1, dtype=torch.int32,
                        device=ids.device)
-    keys, order = kept[:n], kept[n:2 * n]
-    rows = kept[2 * n:3 * n] if bagged else None
-    starts = kept[-V - 1:]
-    with _guard(ids.device):
-        need = lib.ks_token_sort_work(n, V)
-        work = torch.empty(need, dtype=torch.int32, device=ids.device) \
-            if need else None
-        _check(lib.ks_token_sort(
-            ids.data_ptr(), int(ids.dtype == torch.int64), n, V, kind,
-            _ptr(offsets), fixed, bags, keys.data_ptr(), order.data_ptr(),
-            _ptr(rows), starts.data_ptr(), _ptr(work),
-            _raw_stream(ids.device)), "ks_token_sort")
-    return EmbeddingPlan(V, bags, n, order, order if rows is None else rows,
-                         keys, starts)
+    need = lib.ks_token_sort_work(n, V)
+    work = torch.empty(need, dtype=torch.int32, device=ids.device) \
+        if need else None
+    plan = EmbeddingPlan(kept, V, bags, n, bagged)
+    _launch("ks_token_sort", ids.device, ids.data_ptr(),
+            ids.dtype == torch.int64, n, V, kind, _ptr(offsets), fixed, bags,
+            plan._keys, plan._order, plan._rows if bagged else None,
+            plan._starts, _ptr(work))
+    return plan
 
 
 def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
@@ -276,8 +297,7 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
                 raise ValueError("embedding_grad: out overlaps grad")
     if plan.n == 0 or plan.num_bags == 0:
         return out if accumulate else out.zero_()
-    _segment_sum(lib, 1, plan.starts.data_ptr(), 0, plan.num_rows, plan.n,
-                 plan.rows.data_ptr(), 0, plan.num_bags, plan.order.data_ptr(),
-                 weights, plan.keys.data_ptr(), grad, out, scale, accumulate,
-                 "embedding_grad")
+    _segment_sum(lib, 1, plan._starts, 0, plan.num_rows, plan.n, plan._rows, 0,
+                 plan.num_bags, plan._order, weights, plan._keys, grad, out,
+                 scale, accumulate)
     return out

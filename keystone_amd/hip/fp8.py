@@ -15,7 +15,7 @@ from typing import Optional
 
 import torch
 
-from . import _check, _guard, _load, _ptr, _raw_stream
+from . import _launch, _load, _ptr
 
 __all__ = ["Fp8Weight", "fp8_pack", "fp8_linear", "fp8_round"]
 
@@ -92,16 +92,15 @@ def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
     return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _quantise(lib, x: torch.Tensor):
+def _quantise(x: torch.Tensor):
     rows, K = x.shape
     tiles, kb = -(-rows // 16), -(-K // 128)
-    q = torch.empty(tiles, kb, 2048, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(tiles, -(-kb // 4), 64, dtype=torch.uint8,
+    q = torch.empty((tiles, kb, 2048), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((tiles, -(-kb // 4), 64), dtype=torch.uint8,
                          device=x.device)
     pitch = x.stride(0) if rows > 1 else K
-    _check(lib.ks_fp8_quantise(x.data_ptr(), _TYPES[x.dtype], pitch, rows, K,
-                               q.data_ptr(), scales.data_ptr(),
-                               _raw_stream(x.device)), "ks_fp8_quantise")
+    _launch("ks_fp8_quantise", x.device, x.data_ptr(), _TYPES[x.dtype], pitch,
+            rows, K, q.data_ptr(), scales.data_ptr())
     return q, scales
 
 
@@ -111,10 +110,9 @@ def fp8_pack(W: torch.Tensor) -> Fp8Weight:
         raise ValueError(f"fp8_pack.W: expected a matrix, got shape "
                          f"{tuple(W.shape)}")
     if W.is_cuda:
-        lib = _load()
+        _load()
         W = _operand(W.t(), "fp8_pack.W")
-        with _guard(W.device):
-            data, scales = _quantise(lib, W)
+        data, scales = _quantise(W)
         return Fp8Weight(data, scales, W.shape[1], W.shape[0])
     K, N = W.shape
     q, e = _blocks(W.t().to(torch.float32))
@@ -159,13 +157,12 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
         return out
     if K == 0:
         return out.zero_() if bias is None else out.copy_(bias.expand(M, -1))
-    with _guard(X.device):
-        s = lib.ks_fp8_splits(_TYPES[X.dtype], M, W.N, K)
-        q, scales = _quantise(lib, X)
-        part = torch.empty(s, M, W.N, dtype=torch.float32, device=X.device) \
-            if s > 1 else None
-        _check(lib.ks_fp8_gemm(
-            q.data_ptr(), scales.data_ptr(), W.data.data_ptr(),
-            W.scales.data_ptr(), _ptr(bias), out.data_ptr(), _TYPES[X.dtype],
-            _ptr(part), M, K, W.N, _raw_stream(X.device)), "ks_fp8_gemm")
+    q, scales = _quantise(X)
+    kind = _TYPES[X.dtype]
+    s = lib.ks_fp8_splits(kind, M, W.N, K)
+    part = torch.empty(s, M, W.N, dtype=torch.float32, device=X.device) \
+        if s > 1 else None
+    _launch("ks_fp8_gemm", X.device, q.data_ptr(), scales.data_ptr(),
+            W.data.data_ptr(), W.scales.data_ptr(), _ptr(bias),
+            out.data_ptr(), kind, _ptr(part), M, K, W.N)
     return out
