@@ -71,11 +71,10 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _width(D: int, size: int, pitch: int, address: int) -> int:
-    """How many neighbours every row of a matrix can be read by at once: a
-    power of two, 16 bytes at most."""
-    x = (D | pitch) * size | address | 16
-    return max((x & -x) // size, 1)
+def _width(D: int, size: int) -> int:
+    """Elements of a row that a lane reads at once: a power of two, a row's at
+    most and 16 bytes'."""
+    return min(1 << D.bit_length() - 1, 16 // size)
 
 
 def _bags(ids: torch.Tensor, offsets: Optional[torch.Tensor], name: str):
@@ -107,39 +106,27 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     n = ids.numel()
     if n and D:
-        size = table.element_size()
-        pitch = table.stride(0) if V > 1 else D
-        address = table.data_ptr()
         _launch("ks_embedding_lookup", table.device, ids.data_ptr(),
-                ids.dtype == torch.int64, n, address, _TYPES[table.dtype], V,
-                pitch, out.data_ptr(), D, scale,
-                _width(D, size, pitch, address))
+                ids.dtype == torch.int64, n, table.data_ptr(),
+                _TYPES[table.dtype], V, _pitch(table), out.data_ptr(), D,
+                scale, _width(D, table.element_size()))
     return out
 
 
 def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
                  weights, keys, src, out, scale, accumulate):
-    name = "ks_segment_sum"
     D = out.shape[1]
     if count == 0 or D == 0:
         return
-    pitch, out_pitch = _pitch(src), _pitch(out)
-    at, to = src.data_ptr(), out.data_ptr()
-    size, out_size = src.element_size(), out.element_size()
-    # as many as a row of src is read by; out's rows are then written by one
-    # or two stores
-    vec = _width(D, size, pitch, at)
-    x = out_pitch * out_size | to
-    while vec > 1 and x % (vec * out_size):
-        vec //= 2
+    vec = _width(D, src.element_size())
     work = None
     need = lib.ks_segment_work(n, D, vec)
     if need:
         work = torch.empty(need, dtype=torch.float32, device=src.device)
-    _launch(name, src.device, kind, bounds, fixed, count, n, ids, ids_wide, V,
-            order, _ptr(weights), keys, at, _TYPES[src.dtype], pitch, to,
-            _TYPES[out.dtype], out_pitch, _ptr(work), D, scale, accumulate,
-            vec)
+    _launch("ks_segment_sum", src.device, kind, bounds, fixed, count, n, ids,
+            ids_wide, V, order, _ptr(weights), keys, src.data_ptr(),
+            _TYPES[src.dtype], _pitch(src), out.data_ptr(), _TYPES[out.dtype],
+            _pitch(out), _ptr(work), D, scale, accumulate, vec)
 
 
 def embedding_bag(table: torch.Tensor, ids: torch.Tensor,

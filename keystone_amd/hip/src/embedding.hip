@@ -19,27 +19,48 @@ namespace {
 template <typename T, int N>
 using Vec = T __attribute__((ext_vector_type(N)));
 
+// The same in memory, at any element: rows of odd length are read and written
+// 16 bytes at a time like others.
+template <typename T, int N>
+struct InMemory {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+template <typename T, int N, bool PAST = false>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+    using M = typename InMemory<T, N>::type;
+    if constexpr (PAST)
+        return __builtin_nontemporal_load(reinterpret_cast<const M*>(p));
+    else
+        return *reinterpret_cast<const M*>(p);
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void load_row(const T* p, float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = (float)p[0];
-    } else {
-        const Vec<T, N> x = *reinterpret_cast<const Vec<T, N>*>(p);
+    const Vec<T, N> x = load_vec<T, N>(p);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (float)x[i];
-    }
+    for (int i = 0; i < N; ++i) v[i] = (float)x[i];
 }
 
 // PAST: past the caches, for what is too large to be found there later.
 template <typename T, int N, bool PAST = false>
 __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
+    using M = typename InMemory<T, N>::type;
     Vec<T, N> x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (T)v[i];
     if constexpr (PAST)
-        __builtin_nontemporal_store(x, reinterpret_cast<Vec<T, N>*>(p));
+        __builtin_nontemporal_store(x, reinterpret_cast<M*>(p));
     else
-        *reinterpret_cast<Vec<T, N>*>(p) = x;
+        *reinterpret_cast<M*>(p) = x;
+}
+
+// Where lane c of a row begins: at c VEC, the last one early enough to end with
+// the row.  What it then shares with its neighbour both compute alike, and
+// write alike.
+template <int VEC>
+__device__ __forceinline__ int column_of(int c, int D) {
+    return min(c * VEC, D - VEC);
 }
 
 // Token ids as they come: 32 or 64 bits; -1 for one outside the table.
@@ -144,8 +165,7 @@ __device__ __forceinline__ void add_entries(
         for (int u = 0; u < U; ++u) {
             v[u] = V{};
             if (live && row[u] >= 0)
-                v[u] = *reinterpret_cast<const V*>(
-                    src + (long long)row[u] * ld + col);
+                v[u] = load_vec<TS, VEC>(src + (long long)row[u] * ld + col);
             else
                 w[u] = 0.0f;
         }
@@ -168,12 +188,12 @@ __device__ __forceinline__ void add_entries(
 // entry's place and weight, and hands it to the others, so that an entry's
 // index work is done once and not by each lane of its row.  ONCE: no row is
 // read twice, so none is to push others out of the caches.  Places are counted
-// in VEC elements, in 32 bits.  The team is a part of a wave; `waves` of them
+// in 2^unit elements, in 32 bits.  The team is a part of a wave; `waves` of them
 // take turns.
 template <typename TS, int VEC, bool ONCE>
 __device__ __forceinline__ void add_batches(
-        const Entries& t, const TS* src, unsigned pitch, int col, bool live,
-        int b, int e, int g_log, int el_log, int wave, int waves,
+        const Entries& t, const TS* src, unsigned pitch, int unit, int col,
+        bool live, int b, int e, int g_log, int el_log, int wave, int waves,
         float (&acc)[VEC]) {
     using V = Vec<TS, VEC>;
     constexpr unsigned ABSENT = ~0u;
@@ -181,7 +201,7 @@ __device__ __forceinline__ void add_batches(
     const int t_n = 1 << (g_log + el_log), lane = threadIdx.x & 63;
     const int own = lane & (t_n - 1), base = lane - own;
     const int el = own >> g_log, el_n = 1 << el_log;
-    const V* const at = reinterpret_cast<const V*>(src) + col / VEC;
+    const TS* const at = src + col;
     const auto find = [&](int j, unsigned& place, float& w) {
         place = ABSENT;
         w = 1.0f;
@@ -210,7 +230,8 @@ __device__ __forceinline__ void add_batches(
                 f[u] = __shfl(w, base + (k & (t_n - 1)), 64);
                 v[u] = V{};
                 if (live && k < m && p != ABSENT)
-                    v[u] = ONCE ? __builtin_nontemporal_load(at + p) : at[p];
+                    v[u] = load_vec<TS, VEC, ONCE>(
+                        at + ((unsigned long long)p << unit));
                 else
                     f[u] = 0.0f;
             }
@@ -225,10 +246,18 @@ __device__ __forceinline__ void add_batches(
     }
 }
 
+// skip: how many of the columns are the neighbour's, for sums that are added.
 template <typename TO, int VEC>
 __device__ __forceinline__ void put_row(TO* out, const float (&acc)[VEC],
-                                        float scale, int accumulate, int past) {
+                                        float scale, int accumulate, int skip,
+                                        int past) {
     float v[VEC];
+    if (accumulate && skip) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (k >= skip) out[k] = (TO)fmaf(scale, acc[k], (float)out[k]);
+        return;
+    }
     if (accumulate) {
         load_row<TO, VEC>(out, v);
 #pragma unroll
@@ -278,7 +307,8 @@ __device__ __forceinline__ void add_block(float (&acc)[VEC], int g_n,
 struct Cut {
     int g_log, el_log, strip, run_log;
     int cut, chunk, chunks;
-    unsigned pitch;        // src's row pitch in VEC elements; 0: by add_entries
+    unsigned pitch;        // src's row pitch in 2^unit elements; 0: by add_entries
+    int unit;
     int by_entry;          // segments are looked for at entries, not by number
     int dp;                // pitch of part
     float* part;           // [chunks][2][dp]
@@ -306,8 +336,8 @@ __device__ __forceinline__ void add_by_block(const Sum<TS, TO>& a, int col,
                                              bool live, int b, int e,
                                              float (&acc)[VEC]) {
     if (a.c.pitch)
-        add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, col, live, b, e,
-                                   a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6,
+        add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live, b,
+                                   e, a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6,
                                    4, acc);
     else
         add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, b, e,
@@ -330,8 +360,9 @@ template <typename TS, typename TO, int VEC, bool ONCE>
 __device__ void sum_chunk(const Sum<TS, TO>& a, int c, float (*red)[64 * VEC]) {
     __shared__ int found[2][3];
     const int g_n = 1 << a.c.g_log, wave = threadIdx.x >> 6;
-    const int g = threadIdx.x & (g_n - 1);
-    const int col = (blockIdx.y * g_n + g) * VEC;
+    const int place = blockIdx.y * g_n + (threadIdx.x & (g_n - 1));
+    const int col = column_of<VEC>(place, a.D);
+    const bool live = place * VEC < a.D;
     const int i0 = c * a.c.chunk;
     const int i1 = (int)min((long long)a.segs.n, (long long)i0 + a.c.chunk);
     if (wave < 2) {
@@ -348,10 +379,10 @@ __device__ void sum_chunk(const Sum<TS, TO>& a, int c, float (*red)[64 * VEC]) {
     for (int side = 0; side < 2; ++side) {
         if (found[side][0] < 0) continue;
         float acc[VEC] = {};
-        add_by_block<TS, TO, VEC, ONCE>(a, col, col < a.D, found[side][1],
+        add_by_block<TS, TO, VEC, ONCE>(a, col, live, found[side][1],
                                         found[side][2], acc);
         add_block<VEC>(acc, g_n, red);
-        if (threadIdx.x < g_n && col < a.D)
+        if (threadIdx.x < g_n && live)
             store_row<float, VEC>(
                 a.c.part + ((long long)c * 2 + side) * a.c.dp + col, acc);
     }
@@ -411,22 +442,23 @@ void segment_sum_kernel(Sum<TS, TO> a) {
 
     const int g_n = 1 << a.c.g_log, el_n = 1 << a.c.el_log;
     const int team_log = a.c.g_log + a.c.el_log;
-    const int g = threadIdx.x & (g_n - 1);
+    const int place_in_row = blockIdx.y * g_n + (threadIdx.x & (g_n - 1));
     const int block_el = threadIdx.x >> a.c.g_log, block_el_n = 256 >> a.c.g_log;
     const int el = block_el & (el_n - 1);
-    const int col = (blockIdx.y * g_n + g) * VEC;
-    const bool live = col < a.D;
+    const int col = column_of<VEC>(place_in_row, a.D);
+    const bool live = place_in_row * VEC < a.D;
+    const int skip = place_in_row * VEC - col;
     if (empty && live) {
         const float zero[VEC] = {};
         for (int r = block_el; r < a.c.strip; r += block_el_n)
             if (empty >> r & 1)
-                put_row<TO, VEC>(a.out + place(r) * a.ldo + col, zero, 0.0f, 0,
+                put_row<TO, VEC>(a.out + place(r) * a.ldo + col, zero, 0.0f, 0, 0,
                                  a.past);
     }
     for (int k = threadIdx.x >> team_log; k < teams_share; k += 256 >> team_log) {
         float acc[VEC] = {};
         if (a.c.pitch)
-            add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, col, live,
+            add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live,
                                        from[k], to[k], a.c.g_log, a.c.el_log, 0,
                                        1, acc);
         else
@@ -435,7 +467,7 @@ void segment_sum_kernel(Sum<TS, TO> a) {
         add_lanes<VEC>(acc, g_n, g_n * el_n);
         if (live && el == 0)
             put_row<TO, VEC>(a.out + (long long)seg[k] * a.ldo + col, acc,
-                             a.scale, a.accumulate, a.past);
+                             a.scale, a.accumulate, skip, a.past);
     }
 #pragma unroll 1
     for (int k = 63; k > 63 - blocks_share; --k) {
@@ -444,7 +476,7 @@ void segment_sum_kernel(Sum<TS, TO> a) {
         add_block<VEC>(acc, g_n, red);
         if (live && threadIdx.x < g_n)
             put_row<TO, VEC>(a.out + (long long)seg[k] * a.ldo + col, acc,
-                             a.scale, a.accumulate, a.past);
+                             a.scale, a.accumulate, skip, a.past);
     }
 }
 
@@ -460,10 +492,11 @@ void segment_join_kernel(Segs segs, Cut c, TO* __restrict__ out, long long ldo,
     bounds_of(segs, s, b, e);
     const int last = (e - 1) / c.chunk;
     const int g_n = 1 << c.g_log, el_n = 256 >> c.g_log;
-    const int g = threadIdx.x & (g_n - 1), el = threadIdx.x >> c.g_log;
-    const int col = (blockIdx.y * g_n + g) * VEC;
+    const int place = blockIdx.y * g_n + (threadIdx.x & (g_n - 1));
+    const int el = threadIdx.x >> c.g_log, col = column_of<VEC>(place, D);
+    const bool live = place * VEC < D;
     float acc[VEC] = {};
-    if (col < D) {
+    if (live) {
         const float* first = c.part + (long long)blockIdx.x * 2 * c.dp + col;
         if (el == 0) load_row<float, VEC>(first + c.dp, acc);
 #pragma unroll 4
@@ -475,9 +508,9 @@ void segment_join_kernel(Segs segs, Cut c, TO* __restrict__ out, long long ldo,
         }
     }
     add_block<VEC>(acc, g_n, red);
-    if (col < D && threadIdx.x < g_n)
+    if (live && threadIdx.x < g_n)
         put_row<TO, VEC>(out + (long long)s * ldo + col, acc, scale, accumulate,
-                         0);
+                         place * VEC - col, 0);
 }
 
 // The output's vectors in one line, 1024 a block, whatever a row's length:
@@ -485,7 +518,7 @@ void segment_join_kernel(Segs segs, Cut c, TO* __restrict__ out, long long ldo,
 template <typename T, int VEC, bool PAST>
 __global__ __launch_bounds__(256)
 void lookup_kernel(Ids ids, long long vectors, const T* __restrict__ src,
-                   long long ld, T* __restrict__ out, unsigned cols,
+                   long long ld, T* __restrict__ out, int D, unsigned cols,
                    unsigned magic, float scale) {
     using V = Vec<T, VEC>;
     constexpr int N = 4;
@@ -493,17 +526,19 @@ void lookup_kernel(Ids ids, long long vectors, const T* __restrict__ src,
     const long long row0 = first / cols;
     const unsigned rest = (unsigned)(first - row0 * cols);
     V v[N];
+    long long to[N];
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const unsigned at = rest + u * 256 + threadIdx.x;
         // magic: 2^32 / cols, rounded up; exact as long as at cols < 2^32
         const unsigned r = magic ? __umulhi(at, magic) : at / cols;
+        const int col = column_of<VEC>(at - r * cols, D);
+        to[u] = (row0 + r) * D + col;
         v[u] = V{};
         if (first + u * 256 + threadIdx.x < vectors) {
             const int row = row_of(ids, row0 + r);
             if (row >= 0)
-                v[u] = *reinterpret_cast<const V*>(
-                    src + (long long)row * ld + (at - r * cols) * VEC);
+                v[u] = load_vec<T, VEC>(src + (long long)row * ld + col);
         }
     }
 #pragma unroll
@@ -513,7 +548,7 @@ void lookup_kernel(Ids ids, long long vectors, const T* __restrict__ src,
             float f[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) f[k] = (float)v[u][k] * scale;
-            store_row<T, VEC, PAST>(out + i * VEC, f);
+            store_row<T, VEC, PAST>(out + to[u], f);
         }
     }
 }
@@ -563,8 +598,11 @@ int segment_sum(const SumCall& a) {
     c.g_log = lanes_log(a.D, VEC);
     const int slices = (cols + (1 << c.g_log) - 1) >> c.g_log;
     c.chunk = chunk_of(a.D, VEC);
-    const long long span = a.t.ids.rows * (a.ld / VEC);
-    c.pitch = c.g_log >= 3 && span < 0xffffffffll ? (unsigned)(a.ld / VEC) : 0;
+    c.unit = 0;
+    while (c.unit < 6 && a.ld && !(a.ld >> c.unit & 1)) ++c.unit;
+    const long long pitch = a.ld >> c.unit;
+    c.pitch = c.g_log >= 3 && pitch * a.t.ids.rows < 0xffffffffll
+                  ? (unsigned)pitch : 0;
     const bool some_long = a.segs.n > c.chunk &&
                            !(a.segs.kind == 0 && a.segs.fixed <= c.chunk);
     c.chunks = some_long ? (int)(((long long)a.segs.n + c.chunk - 1) / c.chunk) : 0;
@@ -645,7 +683,7 @@ int sum_by_out(const SumCall& c, int out_type, int vec) {
 template <typename T, int VEC>
 int lookup(const Ids& ids, long long n, const void* src, long long ld,
            void* out, int D, float scale, hipStream_t stream) {
-    const unsigned cols = D / VEC;
+    const unsigned cols = (D + VEC - 1) / VEC;
     const long long vectors = n * cols;
     const unsigned magic = cols == 1 || cols > 32768
                                ? 0 : (unsigned)((1ull << 32) / cols) + 1;
@@ -654,7 +692,7 @@ int lookup(const Ids& ids, long long n, const void* src, long long ld,
     auto* kernel = n * D * (long long)sizeof(T) >= LARGE
                        ? lookup_kernel<T, VEC, true> : lookup_kernel<T, VEC, false>;
     kernel<<<(unsigned)((vectors + 1023) / 1024), 256, 0, stream>>>(
-        ids, vectors, (const T*)src, ld, (T*)out, cols, magic, scale);
+        ids, vectors, (const T*)src, ld, (T*)out, D, cols, magic, scale);
     return (int)hipGetLastError();
 }
 
@@ -674,8 +712,8 @@ int lookup_by_width(const Ids& ids, long long n, const void* src, long long ld,
 
 }  // namespace
 
-// Y[n, D] = scale * T[ids], T [V, D] with row pitch ld.  vec: how many
-// elements every row of T and Y can be read by at once.
+// Y[n, D] = scale * T[ids], T [V, D] with row pitch ld.  vec: elements a lane,
+// a power of two, at most D and 16 bytes.
 KS_EXPORT int ks_embedding_lookup(const void* ids, int ids_wide, long long n,
                                   const void* table, int type, long long V,
                                   long long ld, void* out, int D, float scale,
