@@ -30,13 +30,13 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0,
     }
 }
 
-// WIDE: both arrays begin on 16 bytes.
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(256)
 void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long long n,
                     uint32_t threshold, float scale, uint64_t seed,
                     uint64_t step, const long long* __restrict__ step_at) {
-    using V8 = T __attribute__((ext_vector_type(8)));
+    // at any element: views need not begin on 16 bytes
+    typedef T V8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
     if (step_at) step = (uint64_t)*step_at;
     const long long blocks = (n + 7) / 8;
     const long long b = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -45,7 +45,7 @@ void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long long n,
                          (uint32_t)step, (uint32_t)(step >> 32)};
         philox(c, (uint32_t)seed, (uint32_t)(seed >> 32));
         const long long i = b * 8;
-        if (WIDE && i + 8 <= n) {
+        if (i + 8 <= n) {
             V8 v = *reinterpret_cast<const V8*>(x + i);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -72,10 +72,8 @@ int dropout(const void* x, void* y, long long n, uint32_t threshold,
     // one block of eight elements a thread: 180 us for 2^28 bf16, against 220
     // where a grid of 16 blocks a compute unit walks on
     const long long grid = ((n + 7) / 8 + 255) / 256;
-    const bool wide = ((uintptr_t)x | (uintptr_t)y) % 16 == 0;
-    auto* kernel = wide ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-    kernel<<<(unsigned)grid, 256, 0, stream>>>((const T*)x, (T*)y, n, threshold,
-                                               scale, seed, step, step_at);
+    dropout_kernel<T><<<(unsigned)grid, 256, 0, stream>>>(
+        (const T*)x, (T*)y, n, threshold, scale, seed, step, step_at);
     return (int)hipGetLastError();
 }
 

@@ -26,15 +26,20 @@ using i32x8 = int __attribute__((ext_vector_type(8)));
 
 constexpr int CHUNK = 2048;
 
+// N neighbours in memory, at any element.
+template <typename T, int N>
+struct InMemory {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, int left,
-                                      float (&v)[8]) {
-    using V4 = T __attribute__((ext_vector_type(16 / sizeof(T))));
-    if (wide && left >= 8) {
-        constexpr int W = 16 / sizeof(T);
+__device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
+    constexpr int W = 16 / sizeof(T);
+    using M = typename InMemory<T, W>::type;
+    if (left >= 8) {
 #pragma unroll
         for (int q = 0; q < 8 / W; ++q) {
-            const V4 x = reinterpret_cast<const V4*>(p)[q];
+            const M x = reinterpret_cast<const M*>(p + q * W)[0];
 #pragma unroll
             for (int k = 0; k < W; ++k) v[q * W + k] = (float)x[k];
         }
@@ -48,14 +53,13 @@ __device__ __forceinline__ void load8(const T* p, bool wide, int left,
 // bytes, and 127 + the exponent.  The four lanes of a row, 16 apart, share it.
 template <typename T>
 __device__ __forceinline__ int quantise_block(const T* row, int k, int K, int g,
-                                              bool live, bool wide,
-                                              uint32_t (&w)[8]) {
+                                              bool live, uint32_t (&w)[8]) {
     float v[4][8];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int at = k + j * 32 + g * 8;
-        load8(row + at, wide && live, live ? K - at : 0, v[j]);
+        load8(row + at, live ? K - at : 0, v[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
@@ -89,7 +93,7 @@ __device__ __forceinline__ int quantise_block(const T* row, int k, int K, int g,
 template <typename T>
 __global__ __launch_bounds__(256)
 void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
-                         int K, int tiles, int kblocks, int wide,
+                         int K, int tiles, int kblocks,
                          unsigned char* __restrict__ q,
                          unsigned char* __restrict__ scales) {
     const long long chunk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -99,7 +103,7 @@ void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
     const int row = tile * 16 + (lane & 15);
     uint32_t w[8];
     const int e = quantise_block(x + (long long)row * ld, kb * 128, K, lane >> 4,
-                                 row < rows, wide, w);
+                                 row < rows, w);
     unsigned char* to = q + chunk * CHUNK + lane * 16;
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(to + 1024) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -154,14 +158,13 @@ __device__ __forceinline__ f32x4 bias_at(const float* bias, int n, int N) {
 
 template <typename T>
 __device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
-                                              int N, bool wide, f32x4 v) {
+                                              int N, f32x4 v) {
     T* to = y + m * ld + n;
-    if (wide && n + 4 <= N) {
-        using V4 = T __attribute__((ext_vector_type(4)));
-        V4 o;
+    if (n + 4 <= N) {
+        typename InMemory<T, 4>::type o;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
-        *reinterpret_cast<V4*>(to) = o;
+        *reinterpret_cast<typename InMemory<T, 4>::type*>(to) = o;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -173,8 +176,7 @@ __device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
 template <typename T, int TM, int TN>
 __device__ __forceinline__ void store_tiles(const f32x4 (&acc)[TM][TN], T* y,
                                             float* part, const float* bias,
-                                            int m, int n, int M, int N,
-                                            bool wide) {
+                                            int m, int n, int M, int N) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
         const int at = n + j * 16;
@@ -183,14 +185,13 @@ __device__ __forceinline__ void store_tiles(const f32x4 (&acc)[TM][TN], T* y,
 #pragma unroll
             for (int i = 0; i < TM; ++i)
                 if (m + i * 16 < M)
-                    store_columns<float>(part, N, m + i * 16, at, N, N % 4 == 0,
-                                         acc[i][j]);
+                    store_columns<float>(part, N, m + i * 16, at, N, acc[i][j]);
         } else {
             const f32x4 b = bias_at(bias, at, N);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
                 if (m + i * 16 < M)
-                    store_columns<T>(y, N, m + i * 16, at, N, wide, acc[i][j] + b);
+                    store_columns<T>(y, N, m + i * 16, at, N, acc[i][j] + b);
         }
     }
 }
@@ -239,7 +240,7 @@ __device__ __forceinline__ int scale_at(const unsigned* scales, int kq, int tile
 template <typename T, int TM, int TN, bool EXACT>
 __global__ __launch_bounds__(256)
 void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
-                     const float* __restrict__ bias, int wide, int kper) {
+                     const float* __restrict__ bias, int kper) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int mtiles = ks_ceil_div(a.M, 16), ntiles = ks_ceil_div(a.N, 16);
     const int groups = ks_ceil_div(ntiles, TN);
@@ -268,7 +269,7 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
     }
     store_tiles<T, TM, TN>(
         acc, y, part ? part + (long long)blockIdx.y * a.M * a.N : nullptr, bias,
-        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N, wide);
+        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N);
 }
 
 // Few rows, or few columns: a block has one tile of 16 rows by TN of 16
@@ -276,7 +277,7 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
 template <typename T, int TN>
 __global__ __launch_bounds__(1024)
 void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
-                     const float* __restrict__ bias, int wide, int kper) {
+                     const float* __restrict__ bias, int kper) {
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ f32x4 sums[16][TN][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -310,9 +311,9 @@ void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
         if (m >= a.M || n >= a.N) continue;
         if (part)
             store_columns<float>(part + (long long)blockIdx.y * a.M * a.N, a.N,
-                                 m, n, a.N, a.N % 4 == 0, s);
+                                 m, n, a.N, s);
         else
-            store_columns<T>(y, a.N, m, n, a.N, wide, s + bias_at(bias, n, a.N));
+            store_columns<T>(y, a.N, m, n, a.N, s + bias_at(bias, n, a.N));
     }
 }
 
@@ -355,7 +356,7 @@ __device__ __forceinline__ void mfma_here(f32x4& acc, const i32x8& w,
 template <typename T>
 __global__ __launch_bounds__(256, 1)
 void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
-                         const float* __restrict__ bias, int wide, int kper,
+                         const float* __restrict__ bias, int kper,
                          int mblocks, int nblocks) {
     __shared__ __attribute__((aligned(16))) unsigned char
         stage[STAGES][BIG / 16 * CHUNK];
@@ -477,7 +478,7 @@ void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     store_tiles<T, 8, 8>(
         acc, y, part ? part + (long long)split * a.M * a.N : nullptr, bias,
-        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N, wide);
+        m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N);
 }
 
 template <typename T>
@@ -497,10 +498,9 @@ template <typename T>
 int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
              unsigned char* scales, hipStream_t stream) {
     const int tiles = ks_ceil_div(rows, 16), kblocks = ks_ceil_div(K, 128);
-    const int wide = (uintptr_t)x % 16 == 0 && ld * sizeof(T) % 16 == 0;
     const long long chunks = (long long)tiles * kblocks;
     fp8_quantise_kernel<T><<<(unsigned)((chunks + 3) / 4), 256, 0, stream>>>(
-        (const T*)x, ld, rows, K, tiles, kblocks, wide, q, scales);
+        (const T*)x, ld, rows, K, tiles, kblocks, q, scales);
     return (int)hipGetLastError();
 }
 
@@ -552,7 +552,7 @@ int splits_of(int type, int M, int N, int kblocks) {
 }
 
 template <typename T>
-void rows(const Gemm& a, T* y, float* part, const float* bias, int wide,
+void rows(const Gemm& a, T* y, float* part, const float* bias,
           int splits, int kper, hipStream_t stream) {
     const int nt = ks_ceil_div(a.N, 16), mt = ks_ceil_div(a.M, 16);
     // 1021 x 8192 x 147: 12 us with three columns of tiles a block in 32 bits
@@ -562,7 +562,7 @@ void rows(const Gemm& a, T* y, float* part, const float* bias, int wide,
     const int tn = (long long)mt * nt <= 512 ? 1 : WIDE;
     const unsigned grid = (unsigned)mt * ks_ceil_div(nt, tn);
     auto* kernel = tn == 1 ? fp8_rows_kernel<T, 1> : fp8_rows_kernel<T, WIDE>;
-    kernel<<<dim3(grid, splits), 1024, 0, stream>>>(a, y, part, bias, wide, kper);
+    kernel<<<dim3(grid, splits), 1024, 0, stream>>>(a, y, part, bias, kper);
 }
 
 template <typename T>
@@ -570,17 +570,16 @@ int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
          hipStream_t stream) {
     const Kind kind = kind_of(type, a.M, a.N, a.kblocks);
     const int splits = splits_of(type, a.M, a.N, a.kblocks);
-    const int wide = a.N % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
     // splits begin at whole words of scales
     const int kper = ks_ceil_div(ks_ceil_div(a.kblocks, splits), 4) * 4;
     float* parts = splits > 1 ? part : nullptr;
     if (kind == ROWS) {
-        rows<T>(a, (T*)y, parts, bias, wide, splits, kper, stream);
+        rows<T>(a, (T*)y, parts, bias, splits, kper, stream);
     } else if (kind == LARGE) {
         if constexpr (sizeof(T) == 2) {
             const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
             fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
-                a, (T*)y, parts, bias, wide, kper, mb, nb);
+                a, (T*)y, parts, bias, kper, mb, nb);
         }
     } else {
         const int down = tiles_down(a.M, a.N);
@@ -589,7 +588,7 @@ int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
         auto* kernel = down == 2 ? fp8_gemm_kernel<T, 2, 4, sizeof(T) == 4>
                                  : fp8_gemm_kernel<T, 4, 4, sizeof(T) == 4>;
         kernel<<<dim3((unsigned)((waves + 3) / 4), splits), 256, 0, stream>>>(
-            a, (T*)y, parts, bias, wide, kper);
+            a, (T*)y, parts, bias, kper);
     }
     if (splits > 1) {
         const long long n = (long long)a.M * a.N;
