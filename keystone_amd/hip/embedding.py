@@ -26,7 +26,9 @@ __all__ = ["EmbeddingPlan", "embedding_lookup", "embedding_bag",
            "embedding_plan", "embedding_grad"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_MAX = 2 ** 31 - 2
+_MAX_ROWS = 2 ** 31 - 2 ** 16     # of a table that is looked up
+_MAX = 2 ** 29                    # ids, bags and rows of a sum or gradient
+_MAX_DIM = 2 ** 22
 
 
 def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -40,8 +42,9 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name}: expected a matrix, got shape "
                          f"{tuple(t.shape)}")
     rows, D = t.shape
-    if rows > _MAX or D > _MAX:
-        raise ValueError(f"{name}: {tuple(t.shape)} is over {_MAX} a side")
+    if rows > _MAX_ROWS or D > _MAX_DIM:
+        raise ValueError(f"{name}: {tuple(t.shape)} is over {_MAX_ROWS} rows "
+                         f"or {_MAX_DIM} columns")
     if D > 1 and t.stride(1) != 1:
         return t.contiguous()
     return t
@@ -136,8 +139,10 @@ def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
     """``Y[b] = scale * sum_j weights_j table[ids_j]`` over the ids of bag b:
     [bags, D] in the table's type, zeros for an empty bag.
 
-    ``offsets`` [bags + 1], ascending, cut ids [n] into bags; without them
-    ids are [bags, length].  ``weights``: float32, one for each id."""
+    ``offsets`` [bags + 1], ascending, cut ids [n] into bags (ids before the
+    first and behind the last belong to none); without them ids are [bags,
+    length].  ``weights``: float32, one for each id.  At most 2^29 ids and
+    bags."""
     lib = _load()
     table = _matrix(table, "embedding_bag.table")
     ids = _whole(ids, "embedding_bag.ids", table.device)
@@ -176,10 +181,12 @@ class EmbeddingPlan:
         self.device = kept.device
         # keys, order, rows where there are bags, starts: one allocation
         self._kept, self._bagged = kept, bagged
-        self._keys = kept.data_ptr()
-        self._order = self._keys + 4 * n
-        self._rows = self._order + (4 * n if bagged else 0)
-        self._starts = self._rows + 4 * n
+
+    def _places(self):
+        """Where keys, order, rows and starts lie."""
+        at, step = self._kept.data_ptr(), 4 * self.n
+        rows = at + 2 * step if self._bagged else at + step
+        return at, at + step, rows, rows + step
 
     @property
     def keys(self) -> torch.Tensor:
@@ -226,10 +233,10 @@ def embedding_plan(ids: torch.Tensor, num_rows: int,
     work = torch.empty(need, dtype=torch.int32, device=ids.device) \
         if need else None
     plan = EmbeddingPlan(kept, V, bags, n, bagged)
+    keys, order, rows, starts = plan._places()
     _launch("ks_token_sort", ids.device, ids.data_ptr(),
             ids.dtype == torch.int64, n, V, kind, _ptr(offsets), fixed, bags,
-            plan._keys, plan._order, plan._rows if bagged else None,
-            plan._starts, _ptr(work))
+            keys, order, rows if bagged else None, starts, _ptr(work))
     return plan
 
 
@@ -284,7 +291,8 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
                 raise ValueError("embedding_grad: out overlaps grad")
     if plan.n == 0 or plan.num_bags == 0:
         return out if accumulate else out.zero_()
-    _segment_sum(lib, 1, plan._starts, 0, plan.num_rows, plan.n, plan._rows, 0,
-                 plan.num_bags, plan._order, weights, plan._keys, grad, out,
-                 scale, accumulate)
+    keys, order, rows, starts = plan._places()
+    _segment_sum(lib, 1, starts, 0, plan.num_rows, plan.n, rows, 0,
+                 plan.num_bags, order, weights, keys, grad, out, scale,
+                 accumulate)
     return out

@@ -31,7 +31,15 @@ class Fp8Weight:
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, K: int,
                  N: int):
-        self.data, self.scales, self.K, self.N = data, scales, K, N
+        tiles, kb = -(-N // 16), -(-K // 128)
+        for t, shape in ((data, (tiles, kb, 2048)),
+                         (scales, (tiles, -(-kb // 4), 64))):
+            if t.shape != shape or t.dtype != torch.uint8:
+                raise ValueError(f"Fp8Weight: expected uint8 {shape} for W "
+                                 f"[{K}, {N}], got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        self.data, self.scales = data.contiguous(), scales.contiguous()
+        self.K, self.N = K, N
 
     def to(self, device) -> "Fp8Weight":
         return Fp8Weight(self.data.to(device), self.scales.to(device), self.K,
@@ -140,7 +148,7 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
     M, K = X.shape
     if K != W.K:
         raise ValueError(f"fp8_linear: X has {K} columns, W {W.K} rows")
-    if W.data.device != X.device:
+    if W.data.device != X.device or W.scales.device != X.device:
         raise RuntimeError(f"fp8_linear: X is on {X.device}, W on "
                            f"{W.data.device}")
     if bias is not None:

@@ -10,6 +10,14 @@
 // stretch of ids, a token's is its stretch of the sorted tokens, so that
 // every sum has one order and no atomics, and two runs agree bit for bit.
 // Sums are held in 32 bits and rounded once, to the output's type.
+//
+// All of it is memory.  Measured on one MI355X (a large copy: 4.75 TB/s):
+//   lookup of 262144 x 512 bf16 rows of 100000: 54 us, 5 TB/s written
+//   sums of 3.3 M f16 rows of 256 over 32768 bags: 194 us, 8.6 TB/s gathered,
+//     60 % of it from the L2s; half the cycles issue vector instructions
+//   gradient of 1048576 bf16 rows of 256 onto 100000: 137 us, 4.6 TB/s
+//   gradient of 7.8 M weighted entries onto 100000 x 2 f32: 142 us; each
+//     weight, gathered in the sorted order, costs a cache line
 #include "common.h"
 
 #include <cstdint>

@@ -14,6 +14,13 @@
 // Byte t of lane l is element k = 32 (t div 8) + 8 (l div 16) + t mod 8 of
 // row l mod 16: an order of K that quantising reads in whole sectors.  Rows
 // past the end and K past the end are zeros.
+//
+// Measured on one MI355X (a large 8-bit library product: 2.66 PFLOP/s):
+//   quantising 8192 x 65536 bf16: 300 us, 5.4 TB/s read and written
+//   8192 x 65536 x 1000 bf16: 490 us with the join, 2.2 PFLOP/s, the matrix
+//     unit 59 % busy; 8192 x 8192 x 8192: 463 us, 2.37 PFLOP/s
+//   8192 x 8192 x 1000 f32: 175 us, 0.77 PFLOP/s
+//   1 x 16384 x 1000 f32: 7.4 us, 2.3 TB/s of W from 63 blocks
 #include "common.h"
 
 #include <cstdint>

@@ -262,6 +262,19 @@ def test_dtype_limits_and_infinities(hip):
     assert got[5:].eq(0).all()
 
 
+def test_a_copied_plan_outlives_the_first(hip):
+    import copy
+    g = gen(8)
+    ids, dy = some_ids(900, 40, g), torch.randn(900, 24, generator=g).cuda()
+    plan = hip.embedding_plan(ids, 40)
+    want = hip.embedding_grad(dy, plan)
+    again = copy.deepcopy(plan)
+    assert again.starts.data_ptr() != plan.starts.data_ptr()
+    del plan
+    torch.zeros(3000, dtype=torch.int32, device="cuda").fill_(-1)
+    assert torch.equal(hip.embedding_grad(dy, again), want)
+
+
 def test_captured_and_replayed(hip):
     """Lookup, plan and gradient in one graph, replayed on changed inputs."""
     g = gen(6)

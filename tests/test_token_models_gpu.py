@@ -206,7 +206,9 @@ def test_refusals():
         (RuntimeError, lambda: hip.embedding_bag(T, ids, off, w.double())),
         (RuntimeError, lambda: hip.embedding_bag(T, ids, off, w.cpu())),
         (ValueError, lambda: hip.embedding_plan(ids, -1)),
-        (ValueError, lambda: hip.embedding_plan(ids, 2 ** 31 - 1)),
+        (ValueError, lambda: hip.embedding_plan(ids, 2 ** 29 + 1)),
+        (ValueError, lambda: hip.embedding_bag(
+            T, ids[:0, None].expand(0, 3).new_empty(2 ** 29 + 1, 0))),
         (ValueError, lambda: hip.embedding_plan(ids, 6, pooled=True)),
         (ValueError, lambda: hip.embedding_grad(dy[:2], plan)),
         (RuntimeError, lambda: hip.embedding_grad(dy.double(), plan)),
@@ -231,6 +233,9 @@ def test_refusals():
         (ValueError, lambda: hip.dropout(T[:5], 0.5, 0, out=T[1:])),
         (RuntimeError, lambda: hip.fp8_pack(T.double())),
         (ValueError, lambda: hip.fp8_pack(T[None])),
+        (ValueError, lambda: hip.Fp8Weight(W.data, W.scales, 6, 17)),
+        (ValueError, lambda: hip.Fp8Weight(W.data, W.scales, 129, 4)),
+        (ValueError, lambda: hip.Fp8Weight(W.data.int(), W.scales, 6, 4)),
         (ValueError, lambda: hip.fp8_linear(T, W)),
         (RuntimeError, lambda: hip.fp8_linear(T[:, :1].double(), W)),
         (RuntimeError, lambda: hip.fp8_linear(
