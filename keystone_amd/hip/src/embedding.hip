@@ -13,9 +13,9 @@
 //
 // All of it is memory.  Measured on one MI355X (a large copy: 4.75 TB/s):
 //   lookup of 262144 x 512 bf16 rows of 100000: 54 us, 5 TB/s written
-//   sums of 3.3 M f16 rows of 256 over 32768 bags: 194 us, 8.6 TB/s gathered,
-//     60 % of it from the L2s; half the cycles issue vector instructions
-//   gradient of 1048576 bf16 rows of 256 onto 100000: 137 us, 4.6 TB/s
+//   sums of 3.3 M f16 rows of 256 over 32768 bags: 127 us, 13 TB/s gathered,
+//     60 % of it from the L2s
+//   gradient of 1048576 bf16 rows of 256 onto 100000: 136 us, 4.7 TB/s
 //   gradient of 7.8 M weighted entries onto 100000 x 2 f32: 142 us; each
 //     weight, gathered in the sorted order, costs a cache line
 #include "common.h"
@@ -61,6 +61,23 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
         __builtin_nontemporal_store(x, reinterpret_cast<M*>(p));
     else
         *reinterpret_cast<M*>(p) = x;
+}
+
+template <typename T, int N, bool PAST>
+__device__ __forceinline__ Vec<T, N> load_buffer(__amdgpu_buffer_rsrc_t b,
+                                                 unsigned at) {
+    constexpr int BYTES = N * sizeof(T), NT = PAST ? 2 : 0;
+    if constexpr (BYTES == 16)
+        return __builtin_bit_cast(
+            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, NT));
+    else if constexpr (BYTES == 8)
+        return __builtin_bit_cast(
+            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, NT));
+    else if constexpr (BYTES == 4)
+        return __builtin_bit_cast(
+            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, NT));
+    else
+        return Vec<T, N>{};       // not reached: a row of eight lanes is longer
 }
 
 // Where lane c of a row begins: at c VEC, the last one early enough to end with
@@ -254,6 +271,65 @@ __device__ __forceinline__ void add_batches(
     }
 }
 
+// The same through a buffer of up to 2 GB: an entry outside the table has a
+// place outside the buffer, which reads as zeros without a branch, and places
+// are bytes.  Sums of 3.3 M f16 rows of 256 over 32768 bags: 127 us, against
+// 193 us by add_batches, whose 34 vector instructions a load fill half the
+// cycles.
+template <typename TS, int VEC, bool ONCE>
+__device__ __forceinline__ void add_buffered(
+        const Entries& t, const TS* src, unsigned bytes, unsigned pitch, int col,
+        int b, int e, int g_log, int el_log, int wave, int waves,
+        float (&acc)[VEC]) {
+    constexpr unsigned OUTSIDE = 0x80000000u;
+    constexpr int R = 8;          // divides the lanes of a row, eight or more
+    const int t_n = 1 << (g_log + el_log), lane = threadIdx.x & 63;
+    const int own = lane & (t_n - 1), base = lane - own;
+    const int el = own >> g_log, el_n = 1 << el_log;
+    const __amdgpu_buffer_rsrc_t rows =
+        __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, bytes, 0x00020000);
+    const unsigned at = (unsigned)col * sizeof(TS);
+    const auto find = [&](int j, unsigned& place, float& w) {
+        place = OUTSIDE;
+        w = 0.0f;
+        if (j < e) {
+            const int row = row_of(t.ids, j);
+            if (row >= 0) {
+                place = (unsigned)row * pitch;
+                w = t.weights ? t.weights[t.order ? t.order[j] : j] : 1.0f;
+            }
+        }
+    };
+    int i = b + wave * t_n;
+    unsigned place;
+    float w;
+    find(i + own, place, w);
+    for (; i < e; i += waves * t_n) {
+        unsigned next;
+        float wn;
+        find(i + waves * t_n + own, next, wn);
+        const int m = min(t_n, e - i);
+        for (int j = el; j - el < m; j += R * el_n) {
+            Vec<TS, VEC> v[R];
+            float f[R];
+#pragma unroll
+            for (int u = 0; u < R; ++u) {
+                const int from = base + j + u * el_n;
+                const unsigned p = (unsigned)__shfl((int)place, from, 64) + at;
+                f[u] = __shfl(w, from, 64);
+                v[u] = load_buffer<TS, VEC, ONCE>(rows, p);
+            }
+#pragma unroll
+            for (int u = 0; u < R; ++u)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    acc[k] = fmaf(f[u], (float)v[u][k], acc[k]);
+        }
+        place = next;
+        w = wn;
+    }
+}
+
 // skip: how many of the columns are the neighbour's, for sums that are added.
 template <typename TO, int VEC>
 __device__ __forceinline__ void put_row(TO* out, const float (&acc)[VEC],
@@ -315,8 +391,9 @@ __device__ __forceinline__ void add_block(float (&acc)[VEC], int g_n,
 struct Cut {
     int g_log, el_log, strip, run_log;
     int cut, chunk, chunks;
-    unsigned pitch;        // src's row pitch in 2^unit elements; 0: by add_entries
-    int unit;
+    unsigned bytes;        // src's, where it is read through a buffer; else 0
+    unsigned pitch;        // src's row pitch in bytes or in 2^unit elements; 0:
+    int unit;              // by add_entries
     int by_entry;          // segments are looked for at entries, not by number
     int dp;                // pitch of part
     float* part;           // [chunks][2][dp]
@@ -343,7 +420,11 @@ template <typename TS, typename TO, int VEC, bool ONCE>
 __device__ __forceinline__ void add_by_block(const Sum<TS, TO>& a, int col,
                                              bool live, int b, int e,
                                              float (&acc)[VEC]) {
-    if (a.c.pitch)
+    if (a.c.bytes)
+        add_buffered<TS, VEC, ONCE>(a.t, a.src, a.c.bytes, a.c.pitch, col, b, e,
+                                    a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6, 4,
+                                    acc);
+    else if (a.c.pitch)
         add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live, b,
                                    e, a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6,
                                    4, acc);
@@ -397,7 +478,7 @@ __device__ void sum_chunk(const Sum<TS, TO>& a, int c, float (*red)[64 * VEC]) {
 }
 
 template <typename TS, typename TO, int VEC, bool ONCE>
-__global__ __launch_bounds__(256, 6)
+__global__ __launch_bounds__(256, 5)
 void segment_sum_kernel(Sum<TS, TO> a) {
     __shared__ float red[3][64 * VEC];
     // the strip's segments: number, first and last entry; those for a team
@@ -465,7 +546,11 @@ void segment_sum_kernel(Sum<TS, TO> a) {
     }
     for (int k = threadIdx.x >> team_log; k < teams_share; k += 256 >> team_log) {
         float acc[VEC] = {};
-        if (a.c.pitch)
+        if (a.c.bytes)
+            add_buffered<TS, VEC, ONCE>(a.t, a.src, a.c.bytes, a.c.pitch, col,
+                                        from[k], to[k], a.c.g_log, a.c.el_log, 0,
+                                        1, acc);
+        else if (a.c.pitch)
             add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live,
                                        from[k], to[k], a.c.g_log, a.c.el_log, 0,
                                        1, acc);
@@ -611,6 +696,15 @@ int segment_sum(const SumCall& a) {
     const long long pitch = a.ld >> c.unit;
     c.pitch = c.g_log >= 3 && pitch * a.t.ids.rows < 0xffffffffll
                   ? (unsigned)pitch : 0;
+    // through a buffer: up to 2 GB, at whole words
+    const long long bytes =
+        ((a.t.ids.rows - 1) * a.ld + a.D) * (long long)sizeof(TS);
+    c.bytes = 0;
+    if (c.pitch && bytes <= 0x7fffffffll &&
+        ((uintptr_t)a.src | a.ld * sizeof(TS) | a.D * sizeof(TS)) % 4 == 0) {
+        c.bytes = (unsigned)bytes;
+        c.pitch = (unsigned)(a.ld * sizeof(TS));
+    }
     const bool some_long = a.segs.n > c.chunk &&
                            !(a.segs.kind == 0 && a.segs.fixed <= c.chunk);
     c.chunks = some_long ? (int)(((long long)a.segs.n + c.chunk - 1) / c.chunk) : 0;
