@@ -175,7 +175,7 @@ def _register_extra(lib: ctypes.CDLL) -> None:
         lib.ks_embedding_lookup.argtypes = [c_p, c_i, c_l, c_p, c_i, c_l, c_l,
                                             c_p, c_i, c_f, c_i, c_p]
         lib.ks_embedding_lookup.restype = c_i
-        lib.ks_segment_work.argtypes = [c_i, c_i, c_i]
+        lib.ks_segment_work.argtypes = [c_i, c_i, c_i, c_i]
         lib.ks_segment_work.restype = c_l
         lib.ks_segment_sum.argtypes = [
             c_i, c_p, c_i, c_i, c_i, c_p, c_i, c_l, c_p, c_p, c_p, c_p, c_i,
@@ -191,10 +191,11 @@ def _register_extra(lib: ctypes.CDLL) -> None:
         lib.ks_dropout.restype = c_i
         lib.ks_fp8_quantise.argtypes = [c_p, c_i, c_l, c_i, c_i, c_p, c_p, c_p]
         lib.ks_fp8_quantise.restype = c_i
-        lib.ks_fp8_splits.argtypes = [c_i, c_i, c_i, c_i]
-        lib.ks_fp8_splits.restype = c_i
-        lib.ks_fp8_gemm.argtypes = [c_p] * 6 + [c_i, c_p, c_i, c_i, c_i, c_p]
-        lib.ks_fp8_gemm.restype = c_i
+        lib.ks_fp8_work.argtypes = [c_i, c_i, c_i, c_i]
+        lib.ks_fp8_work.restype = c_l
+        lib.ks_fp8_linear.argtypes = [c_p, c_i, c_l] + [c_p] * 4 + \
+            [c_i] * 3 + [c_p, c_p]
+        lib.ks_fp8_linear.restype = c_i
     except AttributeError:
         pass
 

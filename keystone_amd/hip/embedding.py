@@ -123,7 +123,7 @@ def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
         return
     vec = _width(D, src.element_size())
     work = None
-    need = lib.ks_segment_work(n, D, vec)
+    need = lib.ks_segment_work(n, D, vec, keys is not None)
     if need:
         work = torch.empty(need, dtype=torch.float32, device=src.device)
     _launch("ks_segment_sum", src.device, kind, bounds, fixed, count, n, ids,

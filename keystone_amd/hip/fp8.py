@@ -165,12 +165,11 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
         return out
     if K == 0:
         return out.zero_() if bias is None else out.copy_(bias.expand(M, -1))
-    q, scales = _quantise(X)
     kind = _TYPES[X.dtype]
-    s = lib.ks_fp8_splits(kind, M, W.N, K)
-    part = torch.empty(s, M, W.N, dtype=torch.float32, device=X.device) \
-        if s > 1 else None
-    _launch("ks_fp8_gemm", X.device, q.data_ptr(), scales.data_ptr(),
-            W.data.data_ptr(), W.scales.data_ptr(), _ptr(bias),
-            out.data_ptr(), kind, _ptr(part), M, K, W.N)
+    work = torch.empty(lib.ks_fp8_work(kind, M, K, W.N), dtype=torch.uint8,
+                       device=X.device)
+    _launch("ks_fp8_linear", X.device, X.data_ptr(), kind,
+            X.stride(0) if M > 1 else K, W.data.data_ptr(),
+            W.scales.data_ptr(), _ptr(bias), out.data_ptr(), M, K, W.N,
+            work.data_ptr())
     return out

@@ -679,7 +679,11 @@ int lanes_log(int D, int vec) {
     if (cols > 64 && (cols + 31) / 32 * 5 <= (cols + 63) / 64 * 8) return 5;
     return log2_up(cols, 6);
 }
-int chunk_of(int D, int vec) {
+// A gradient of up to 1024 tokens has none: the calls for 777 of 100 f32 take
+// 20.8 us without the join's launch and 25.7 us with it.  Where all 1024 are one
+// token, of 512 f32, its block takes 24 us alone, against 14 us.
+int chunk_of(int D, int vec, int n, bool sorted) {
+    if (sorted && n <= 1024) return 1024;
     const int c = 8192 >> lanes_log(D, vec);
     return c < 512 ? c : 512;
 }
@@ -690,7 +694,7 @@ int segment_sum(const SumCall& a) {
     Cut c;
     c.g_log = lanes_log(a.D, VEC);
     const int slices = (cols + (1 << c.g_log) - 1) >> c.g_log;
-    c.chunk = chunk_of(a.D, VEC);
+    c.chunk = chunk_of(a.D, VEC, a.segs.n, a.t.keys);
     c.unit = 0;
     while (c.unit < 6 && a.ld && !(a.ld >> c.unit & 1)) ++c.unit;
     const long long pitch = a.ld >> c.unit;
@@ -830,8 +834,9 @@ KS_EXPORT int ks_embedding_lookup(const void* ids, int ids_wide, long long n,
 }
 
 // How many floats of workspace a segmented sum of n entries needs.
-KS_EXPORT long long ks_segment_work(int n, int D, int vec) {
-    const int chunk = chunk_of(D, vec);
+// sorted: entries come with keys.
+KS_EXPORT long long ks_segment_work(int n, int D, int vec, int sorted) {
+    const int chunk = chunk_of(D, vec, n, sorted);
     if (n <= chunk) return 0;
     return ((long long)n + chunk - 1) / chunk * (2 * ((D + 7) & ~7) + 1);
 }

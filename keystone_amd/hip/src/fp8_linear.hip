@@ -607,6 +607,21 @@ int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
     return (int)hipGetLastError();
 }
 
+// Where a call's workspace has what.
+struct Work {
+    long long scales, part, bytes;
+};
+
+Work work_of(int type, int M, int K, int N) {
+    const long long tiles = ks_ceil_div(M, 16), kb = ks_ceil_div(K, 128);
+    const int splits = splits_of(type, M, N, (int)kb);
+    Work w;
+    w.scales = tiles * kb * CHUNK;
+    w.part = (w.scales + tiles * ((kb + 3) / 4) * 64 + 255) / 256 * 256;
+    w.bytes = w.part + (splits > 1 ? 4ll * splits * M * N : 0);
+    return w;
+}
+
 }  // namespace
 
 // q: 16 ceil(rows/16) x 128 ceil(K/128) bytes, scales: 64 bytes for every 16
@@ -622,19 +637,27 @@ KS_EXPORT int ks_fp8_quantise(const void* x, int type, long long ld, int rows,
     }
 }
 
-// How many [M, N] float32 parts ks_fp8_gemm needs; 1: none.
-KS_EXPORT int ks_fp8_splits(int type, int M, int N, int K) {
-    return splits_of(type, M, N, ks_ceil_div(K, 128));
+// Bytes of workspace that ks_fp8_linear needs: X quantised, its scales, and
+// the splits' parts.
+KS_EXPORT long long ks_fp8_work(int type, int M, int K, int N) {
+    const Work w = work_of(type, M, K, N);
+    return w.bytes;
 }
 
-// y [M, N] = X W + bias of quantised operands; y's type as above, bias may be
-// null.
-KS_EXPORT int ks_fp8_gemm(const unsigned char* xq, const unsigned* xs,
-                          const unsigned char* wq, const unsigned* ws,
-                          const float* bias, void* y, int type, float* part,
-                          int M, int K, int N, hipStream_t stream) {
+// y [M, N] = X W + bias: x [M, K] with row pitch ld and y of one type (as
+// above), bias float32 or null, K > 0.
+KS_EXPORT int ks_fp8_linear(const void* x, int type, long long ld,
+                            const unsigned char* wq, const unsigned* ws,
+                            const float* bias, void* y, int M, int K, int N,
+                            unsigned char* work, hipStream_t stream) {
     if (M == 0 || N == 0) return 0;
-    const Gemm a{xq, xs, wq, ws, M, N, ks_ceil_div(K, 128)};
+    const Work w = work_of(type, M, K, N);
+    const int code = ks_fp8_quantise(x, type, ld, M, K, work, work + w.scales,
+                                     stream);
+    if (code) return code;
+    const Gemm a{work, (const unsigned*)(work + w.scales), wq, ws, M, N,
+                 ks_ceil_div(K, 128)};
+    float* part = (float*)(work + w.part);
     switch (type) {
         case 0: return gemm<float>(a, y, part, bias, type, stream);
         case 1: return gemm<__bf16>(a, y, part, bias, type, stream);
