@@ -17,9 +17,10 @@
 //
 // Measured on one MI355X (a large 8-bit library product: 2.66 PFLOP/s):
 //   quantising 8192 x 65536 bf16: 300 us, 5.4 TB/s read and written
-//   8192 x 65536 x 1000 bf16: 490 us with the join, 2.2 PFLOP/s, the matrix
-//     unit 59 % busy; 8192 x 8192 x 8192: 463 us, 2.37 PFLOP/s
-//   8192 x 8192 x 1000 f32: 175 us, 0.77 PFLOP/s
+//   8192 x 65536 x 1000 bf16: 456 us with the join, 2.35 PFLOP/s, the matrix
+//     unit 59 % busy
+//   8192 x 65536 x 1000 f32: 845 us, 1.27 PFLOP/s (a large bfloat16 library
+//     product: 1.20)
 //   1 x 16384 x 1000 f32: 7.4 us, 2.3 TB/s of W from 63 blocks
 #include "common.h"
 
@@ -324,10 +325,10 @@ void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
     }
 }
 
-// Large products with 16-bit results: a block of four waves has 256 x 256
-// outputs, a wave 128 x 128 of them in 256 accumulator registers, and runs
-// alone on its SIMD.  Per 128 of K and wave that is 64 matrix instructions of
-// 32 cycles.  W's chunks go to LDS (four stages of 32 KB, three steps ahead),
+// Large products: a block of four waves has 256 x 256 outputs, a wave 128 x 128
+// of them in 256 accumulator registers, and runs alone on its SIMD.  Per 128 of
+// K and wave that is 64 matrix instructions of 32 cycles, or 256 of 16 in
+// bfloat16.  W's chunks go to LDS (four stages of 32 KB, three steps ahead),
 // for both waves that need them; X's go straight to registers, each again as
 // soon as its last use is past, so that they have a whole step to arrive.
 // One barrier a step, in its middle: it ends the writing of the next stage
@@ -358,6 +359,25 @@ __device__ __forceinline__ void mfma_here(f32x4& acc, const i32x8& w,
         asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                      "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
                      : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
+}
+
+// The same in bfloat16.  WAIT: an operand may just have been widened, which the
+// matrix unit sees two cycles later.
+template <bool WAIT>
+__device__ __forceinline__ void mfma_here(f32x4& acc, const bf16x8& w,
+                                          const bf16x8& x) {
+    if constexpr (WAIT)
+        asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+                     : "+a"(acc) : "v"(w), "v"(x) : "memory");
+    else
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+                     : "+a"(acc) : "v"(w), "v"(x) : "memory");
+}
+
+// What is made of v from here on is made here: the compiler would widen all of
+// it in front and run out of registers.
+__device__ __forceinline__ void not_before(i32x8& v) {
+    asm volatile("" : "+v"(v));
 }
 
 template <typename T>
@@ -450,22 +470,57 @@ void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
 #pragma unroll
     for (int j = 0; j < 8; ++j) w[j] = read_w(j, k0);
 
+    // what this wave put into stage kb + 1 has arrived: 48 loads or more were
+    // issued since
+    const auto arrive = [&]() {
+        asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
     const auto step = [&](auto q, int kb) {
         fetch_w(kb + STAGES - 1);
+        if constexpr (sizeof(T) == 4) {
+            int xk[8], wk[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                mfma_here<q.value>(acc[i][j], w[j], x[i], ws[j], xs[i]);
-                if (i == 7) w[j] = read_w(j, kb + 1);
+            for (int i = 0; i < 8; ++i) {
+                xk[i] = xs[i] >> 8 * q.value & 255;
+                wk[i] = ws[i] >> 8 * q.value & 255;
             }
-            x[i] = fetch_x(i, kb + 1);
-            if (i == 3) {
-                // what this wave put into stage kb + 1 has arrived: 56 loads
-                // or more were issued since
-                asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                bf16x8 wide[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    not_before(w[j]);
+                    wide[j] = widen(w[j][2 * s], w[j][2 * s + 1], wk[j]);
+                    if (s == 3) w[j] = read_w(j, kb + 1);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    not_before(x[i]);
+                    const bf16x8 v = widen(x[i][2 * s], x[i][2 * s + 1], xk[i]);
+                    mfma_here<true>(acc[i][0], wide[0], v);
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) {
+                        if (i == 0)
+                            mfma_here<true>(acc[i][j], wide[j], v);
+                        else
+                            mfma_here<false>(acc[i][j], wide[j], v);
+                    }
+                    if (s == 3) x[i] = fetch_x(i, kb + 1);
+                }
+                if (s == 1) arrive();
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    mfma_here<q.value>(acc[i][j], w[j], x[i], ws[j], xs[i]);
+                    if (i == 7) w[j] = read_w(j, kb + 1);
+                }
+                x[i] = fetch_x(i, kb + 1);
+                if (i == 3) arrive();
             }
         }
     };
@@ -518,12 +573,14 @@ Kind kind_of(int type, int M, int N, int kblocks) {
     const int mt = ks_ceil_div(M, 16), nt = ks_ceil_div(N, 16);
     if (mt == 1 || (long long)mt * nt <= 512 || (mt <= 64 && nt <= 16))
         return ROWS;
-    // at least four steps for each compute unit.  2048 x 2048 x 2048 bf16 has
-    // four: 37 us against 38 us by TILES; 8192 x 1024 x 2000 eight: 39 against
-    // 53; 512 x 65536 x 1000 sixteen: 59 against 87; 1024 x 4096 x 1000 two:
-    // 38 against 28
-    if (type != 0 && M >= 192 && N >= 192 && kblocks >= 8 &&
-        (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG) * kblocks >= 1024)
+    // At least four steps for each compute unit, eight of the longer ones for
+    // 32-bit results.  bf16: 2048 x 2048 x 2048 has four, 37 us against 38 us by
+    // TILES; 8192 x 1024 x 2000 eight, 39 against 53; 1024 x 4096 x 1000 two,
+    // 38 against 28.  f32: 512 x 16384 x 1000 four, 44 against 33; 8192 x 1024 x
+    // 2000 eight, 47 against 55; 8192 x 8192 x 1000 sixteen, 135 against 174.
+    if (M >= 192 && N >= 192 && kblocks >= 8 &&
+        (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG) * kblocks >=
+            (type == 0 ? 2048 : 1024))
         return LARGE;
     return TILES;
 }
@@ -583,11 +640,9 @@ int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
     if (kind == ROWS) {
         rows<T>(a, (T*)y, parts, bias, splits, kper, stream);
     } else if (kind == LARGE) {
-        if constexpr (sizeof(T) == 2) {
-            const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
-            fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
-                a, (T*)y, parts, bias, kper, mb, nb);
-        }
+        const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
+        fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
+            a, (T*)y, parts, bias, kper, mb, nb);
     } else {
         const int down = tiles_down(a.M, a.N);
         const long long waves = (long long)ks_ceil_div(a.N, 64) *

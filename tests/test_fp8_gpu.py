@@ -109,7 +109,7 @@ def test_linear(hip, dtype, M, K, N):
     assert torch.equal(got, hip.fp8_linear(X, packed))
 
 
-@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N", [
     (2100, 2176, 1030), (1500, 2049, 1600), (8192, 2560, 192),
     (1025, 4224, 2050), (8200, 8192, 1000)])
