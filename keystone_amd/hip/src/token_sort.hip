@@ -3,40 +3,47 @@
 // order of their positions.
 //
 // Radix sort from the lowest digit, at most nine bits a digit.  A digit's
-// pass counts the digits of every tile of 2048 tokens, scans the counts over
-// the tiles, and moves each token to its digit's place.  Inside a wave the
-// tokens of one digit are found by a ballot over each of its bits, so that
-// equal digits keep their order without atomics.  A tile is put in order in
-// LDS first, so that what it writes of one digit is one run.
+// pass counts the digits of every tile of tokens, scans the counts over the
+// tiles, and moves each token to its digit's place.  Inside a wave the tokens
+// of one digit are found by a ballot over each of its bits, so that equal
+// digits keep their order without atomics.  A tile is put in order in LDS
+// first, so that what it writes of one digit is one run.  Up to 8192 tokens
+// each one's place is counted instead, in one launch.
 //
-// Bound by latency and launches: 1048576 tokens of 100000 take 57 us in eight
-// launches (78 us with scattered writes of 4 bytes), 8388608 take 198 us, 777
-// take 12 us in two.
+// Bound by latency and launches, tokens of 100000: 777 take 4.7 us, 4096 take
+// 8.2 us, 16384 take 29 us in seven launches, 1048576 take 56 us (78 us with
+// scattered writes of 4 bytes), 8388608 take 198 us.
 #include "common.h"
 
 #include <cstdint>
 
 namespace {
 
-constexpr int TILE = 2048, WAVES = 4, ROUNDS = TILE / (WAVES * 64);
+constexpr int WAVES = 4;
+// A tile's tokens are so many for each of its block's threads.  Few of them
+// fill the card with few tokens: 65536 take 32 us with two a thread, 53 us
+// with eight, 262144 take 38 and 42 us, 400000 take 49 and 44 us.
+constexpr int FEW = 2, MANY = 8;
+constexpr int ROUNDS_LIMIT = 262144;
+
+int rounds_of(int n) { return n <= ROUNDS_LIMIT ? FEW : MANY; }
+
 constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 
-// The bag of position i: -1 where the bounds leave it out.  lo, hi: a bag that
-// begins at or before i, and one after it or `bags`.
-__device__ __forceinline__ int bag_of(const void* bounds, int kind, int fixed,
-                                      int bags, int i, int lo, int hi) {
-    if (kind == 0) return i / fixed;
-    if (bags == 0) return -1;
-    auto at = [&](int k) -> long long {
+// Bounds of bags, and which positions are in some bag.
+struct Bags {
+    const void* bounds;
+    int kind, fixed, count;  // kind 0: fixed length, 1: int32, 2: int64 bounds
+    __device__ __forceinline__ long long at(int k) const {
         return kind == 1 ? (long long)((const int*)bounds)[k]
                          : ((const long long*)bounds)[k];
-    };
-    while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        if (at(mid) <= i) lo = mid; else hi = mid;
     }
-    return (at(lo) <= i && i < at(lo + 1)) ? lo : -1;
-}
+    __device__ __forceinline__ void inside(int n, long long& from,
+                                           long long& to) const {
+        from = kind ? (count ? at(0) : n) : 0;
+        to = kind && count ? at(count) : n;
+    }
+};
 
 // What a pass reads: the token ids themselves, or (key, position) pairs.  A
 // key is the id, or V for one outside the table or outside every bag.
@@ -44,7 +51,7 @@ struct Source {
     const int2* pairs;
     const void* ids;
     int wide, n, V;
-    const int* bag;    // the positions' bags, where there are bags
+    int* bag;          // the positions' bags, where there are bags
 };
 
 __device__ __forceinline__ int2 pair_at(const Source& s, int i) {
@@ -56,43 +63,97 @@ __device__ __forceinline__ int2 pair_at(const Source& s, int i) {
     return make_int2(key, i);
 }
 
-__global__ __launch_bounds__(256)
-void position_bags_kernel(const void* __restrict__ bounds, int kind, int fixed,
-                          int bags, int n, int* __restrict__ bag) {
-    // the bags of the block's ends, then each position's between them
-    __shared__ int ends[2];
-    const long long first = (long long)blockIdx.x * TILE;
-    if (kind && bags && (threadIdx.x & 63) == 0 && threadIdx.x < 128) {
-        const bool last = threadIdx.x;
-        const long long i = last ? min(first + TILE, (long long)n) - 1 : first;
-        int lo = 0, hi = bags;
+// Inclusive maxima over the block's 256 threads.
+__device__ __forceinline__ int max_block(int x, int* wave_max) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d, 64);
+        if (lane >= d) x = max(x, y);
+    }
+    if (lane == 63) wave_max[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) x = max(x, wave_max[w]);
+    return x;
+}
+
+// The bags of a tile's positions, -1 outside: every bag that begins in the tile
+// marks its first position, and a position's bag is the last mark so far.
+// 524288 tokens in bags of ten are sorted in 59 us, in 69 us where each
+// position searches the bounds.
+template <int ROUNDS>
+__device__ __forceinline__ void bags_of_tile(const Bags& bags, int n,
+                                             long long first,
+                                             int* __restrict__ bag) {
+    constexpr int TILE = ROUNDS * 256;
+    __shared__ int mark[TILE], ends[2], wave_max[4];
+    const int tid = threadIdx.x;
+    if (bags.kind == 0) {
+        for (int r = 0; r < ROUNDS; ++r) {
+            const long long i = first + r * 256 + tid;
+            if (i < n) bag[i] = (int)i / bags.fixed;
+        }
+        return;
+    }
+    for (int r = 0; r < ROUNDS; ++r) mark[r * 256 + tid] = 0;
+    // the last bags that begin at or before the tile's ends
+    if (bags.count && (tid & 63) == 0 && tid < 128) {
+        const long long i = tid ? first + TILE - 1 : first;
+        int lo = 0, hi = bags.count;
         while (hi - lo > 1) {
             const int mid = lo + (hi - lo) / 2;
-            const long long v = kind == 1 ? (long long)((const int*)bounds)[mid]
-                                          : ((const long long*)bounds)[mid];
-            if (v <= i) lo = mid; else hi = mid;
+            if (bags.at(mid) <= i) lo = mid; else hi = mid;
         }
-        ends[last] = lo + last;
+        ends[tid >> 6] = lo;
     }
     __syncthreads();
-    for (int r = 0; r < TILE / 256; ++r) {
-        const long long i = first + r * 256 + threadIdx.x;
-        if (i < n)
-            bag[i] = bag_of(bounds, kind, fixed, bags, (int)i, ends[0], ends[1]);
+    if (bags.count)
+        for (int b = ends[0] + tid; b <= ends[1]; b += 256) {
+            const long long i = max(bags.at(b), first) - first;
+            if (i < TILE) atomicMax(&mark[i], b);
+        }
+    __syncthreads();
+    int last[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        last[r] = mark[tid * ROUNDS + r];
+        if (r) last[r] = max(last[r], last[r - 1]);
+    }
+    const int here = max_block(last[ROUNDS - 1], wave_max);
+    int before = __shfl_up(here, 1, 64);
+    if ((tid & 63) == 0) {
+        before = 0;
+        for (int w = 0; w < tid >> 6; ++w) before = max(before, wave_max[w]);
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        mark[tid * ROUNDS + r] = max(before, last[r]);
+    __syncthreads();
+    long long from, to;
+    bags.inside(n, from, to);
+    for (int r = 0; r < ROUNDS; ++r) {
+        const long long i = first + r * 256 + tid;
+        if (i < n) bag[i] = i >= from && i < to ? mark[r * 256 + tid] : -1;
     }
 }
 
+// The first pass finds the positions' bags too.
+template <int ROUNDS>
 __global__ __launch_bounds__(256)
 void digit_count_kernel(Source src, int shift, int bits,
-                        int* __restrict__ counts, int tiles) {
+                        int* __restrict__ counts, int tiles, Bags bags) {
     __shared__ int bin[MAX_BINS];
     const int bins = 1 << bits;
+    const long long first = (long long)blockIdx.x * (ROUNDS * 256);
     for (int i = threadIdx.x; i < bins; i += 256) bin[i] = 0;
+    // a thread reads the bags that it has written itself
+    if (src.bag && !src.pairs) bags_of_tile<ROUNDS>(bags, src.n, first, src.bag);
     __syncthreads();
-    const int first = blockIdx.x * TILE;
-    for (int r = 0; r < TILE / 256; ++r) {
-        const int i = first + r * 256 + threadIdx.x;
-        if (i < src.n) atomicAdd(&bin[(pair_at(src, i).x >> shift) & (bins - 1)], 1);
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const long long i = first + r * 256 + threadIdx.x;
+        if (i < src.n)
+            atomicAdd(&bin[(pair_at(src, (int)i).x >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < bins; i += 256)
@@ -177,12 +238,14 @@ __device__ __forceinline__ int scan_block(int x, int* wave_sum) {
 }
 
 // The last pass (pairs_out null) writes keys, order and rows.
+template <int ROUNDS>
 __global__ __launch_bounds__(256)
 void digit_move_kernel(Source src, int shift, int bits,
                        const int* __restrict__ counts, int tiles,
                        const int* __restrict__ totals,
                        int2* __restrict__ pairs_out, int* __restrict__ keys,
                        int* __restrict__ order, int* __restrict__ rows) {
+    constexpr int TILE = ROUNDS * 256;
     __shared__ int count[WAVES][MAX_BINS];
     __shared__ int there[MAX_BINS];   // global less local place of a digit
     __shared__ int2 sorted[TILE];
@@ -256,106 +319,105 @@ void digit_move_kernel(Source src, int shift, int bits,
     }
 }
 
-// Up to SMALL tokens: one block sorts them in LDS, all digits in one launch.
-// Each of its waves has four rounds of 64 tokens.
-constexpr int SMALL = 4096, SMALL_ROUNDS = 4;
+// Up to SMALL tokens, in one launch: a token's place is how many tokens sort
+// before it, counted against all of them in LDS by 16 lanes.  n^2 comparisons
+// are less than the passes' barriers: two instructions each, over the whole
+// card.  Further blocks count the tokens below each of STARTS ids.  8192
+// tokens take 15 us, 29 us by digits; 16384 take 77 and 29 us.
+constexpr int SMALL = 8192, PLACED = 16, STARTS = 2048;
 
-template <int SMALL_WAVES>
-__global__ __launch_bounds__(64 * SMALL_WAVES)
+__global__ __launch_bounds__(256)
 void small_sort_kernel(const void* __restrict__ ids, int wide, int n, int V,
-                       const void* __restrict__ bounds, int kind, int fixed,
-                       int bags, int bits, int passes, int* __restrict__ keys,
-                       int* __restrict__ order, int* __restrict__ rows) {
-    constexpr int THREADS = 64 * SMALL_WAVES, MOST = THREADS * SMALL_ROUNDS;
-    __shared__ int key_at[MOST], from_at[MOST];
-    __shared__ int count[SMALL_WAVES][MAX_BINS];
-    __shared__ int wave_sum[SMALL_WAVES];
-    // digits a thread
-    constexpr int EACH = THREADS < MAX_BINS ? MAX_BINS / THREADS : 1;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int bins = 1 << bits;
-    const int first = wave * (SMALL_ROUNDS * 64) + lane;
-    int key[SMALL_ROUNDS], from[SMALL_ROUNDS], rank[SMALL_ROUNDS];
+                       Bags bags, int* __restrict__ keys,
+                       int* __restrict__ order, int* __restrict__ rows,
+                       int* __restrict__ starts, int placing) {
+    __shared__ __attribute__((aligned(16))) int key_at[SMALL];
+    __shared__ int wave_sum[4];
+    const int tid = threadIdx.x;
+    long long from, to;
+    bags.inside(n, from, to);
+    auto key_of = [&](int i) -> int {
+        const long long v = wide ? ((const long long*)ids)[i]
+                                 : (long long)((const int*)ids)[i];
+        return v >= 0 && v < V && i >= from && i < to ? (int)v : V;
+    };
+
+    if ((int)blockIdx.x >= placing) {
+        int* const bin = key_at;
+        const long long v0 = (long long)(blockIdx.x - placing) * STARTS;
+        for (int i = tid; i < STARTS; i += 256) bin[i] = 0;
+        __syncthreads();
+        int below = 0;
+#pragma unroll 4
+        for (int i = tid; i < n; i += 256) {
+            const long long at = key_of(i) - v0;
+            if (at < 0) ++below;
+            else if (at < STARTS) atomicAdd(&bin[at], 1);
+        }
+        __syncthreads();
+        // eight ids a thread, then what lies below them
+        constexpr int EACH = STARTS / 256;
+        int x[EACH], all = 0;
 #pragma unroll
-    for (int r = 0; r < SMALL_ROUNDS; ++r) {
-        const int i = first + r * 64;
-        from[r] = i;
-        key[r] = V;
-        if (i < n) {
-            const long long v = wide ? ((const long long*)ids)[i]
-                                     : (long long)((const int*)ids)[i];
-            if (v >= 0 && v < V) key[r] = (int)v;
-            if (rows && bag_of(bounds, kind, fixed, bags, i, 0, bags) < 0) key[r] = V;
+        for (int q = 0; q < EACH; ++q) {
+            x[q] = all;
+            all += bin[tid * EACH + q];
+        }
+        const int mine = scan_block(all, wave_sum);
+#pragma unroll
+        for (int d = 32; d; d >>= 1) below += __shfl_xor(below, d, 64);
+        if ((tid & 63) == 0) wave_sum[tid >> 6] = below;
+        __syncthreads();
+        below = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+#pragma unroll
+        for (int q = 0; q < EACH; ++q) bin[tid * EACH + q] = below + mine + x[q];
+        __syncthreads();
+        for (int i = tid; i < STARTS; i += 256)
+            if (v0 + i <= V) starts[v0 + i] = bin[i];
+        return;
+    }
+
+    const int part = tid & 15, i = blockIdx.x * PLACED + (tid >> 4);
+    const int groups = (n + 3) / 4;
+#pragma unroll 4
+    for (int j = tid; j < groups * 4; j += 256)
+        key_at[j] = j < n ? key_of(j) : 0x7fffffff;
+    // the token's bag, the last that begins at or before it: 16 bounds a step
+    int row = 0;
+    if (rows) {
+        if (bags.kind == 0) {
+            row = min(i, n - 1) / bags.fixed;
+        } else if (bags.count) {
+            int lo = 0, hi = bags.count;
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 15) / 16;
+                const int k = lo + part * step;
+                const unsigned long long at =
+                    __ballot(k < hi && bags.at(k) <= i);
+                const int c = __popcll(at >> (tid & 48) & 0xffff);
+                if (c) lo += (c - 1) * step;
+                hi = min(hi, lo + step);
+            }
+            row = lo;
         }
     }
-    for (int p = 0; p < passes; ++p) {
-        const int shift = p * bits;
-        for (int i = tid; i < SMALL_WAVES * MAX_BINS; i += THREADS)
-            (&count[0][0])[i] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r)
-            rank[r] = rank_digit((key[r] >> shift) & (bins - 1), bits,
-                                 first + r * 64 < n, count[wave]);
-        __syncthreads();
-        // where each wave's tokens of each digit go
-        int total[EACH], all = 0, s = 0;
-        if (tid < MAX_BINS / EACH) {
-#pragma unroll
-            for (int q = 0; q < EACH; ++q) {
-                total[q] = 0;
-                for (int w = 0; w < SMALL_WAVES; ++w)
-                    total[q] += count[w][tid * EACH + q];
-                all += total[q];
-            }
-            s = all;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int y = __shfl_up(s, d, 64);
-                if (lane >= d) s += y;
-            }
-            if (lane == 63) wave_sum[wave] = s;
-        }
-        __syncthreads();
-        if (tid < MAX_BINS / EACH) {
-            int at = s - all;
-            for (int w = 0; w < wave; ++w) at += wave_sum[w];
-#pragma unroll
-            for (int q = 0; q < EACH; ++q)
-                for (int w = 0; w < SMALL_WAVES; ++w) {
-                    const int c = count[w][tid * EACH + q];
-                    count[w][tid * EACH + q] = at;
-                    at += c;
-                }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r) {
-            if (first + r * 64 < n) {
-                const int to = count[wave][(key[r] >> shift) & (bins - 1)] + rank[r];
-                key_at[to] = key[r];
-                from_at[to] = from[r];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SMALL_ROUNDS; ++r) {
-            const int i = first + r * 64;
-            if (i < n) {
-                key[r] = key_at[i];
-                from[r] = from_at[i];
-            }
-        }
+    __syncthreads();
+    if (i >= n) return;
+    const int key = key_at[i], own = i >> 2;
+    int place = 0;
+#pragma unroll 4
+    for (int g = part; g < groups; g += 16) {
+        const int4 k = *(const int4*)(key_at + g * 4);
+        const int most = g < own ? key + 1 : key;
+        place += (k.x < most) + (k.y < most) + (k.z < most) + (k.w < most);
     }
+    if (part < (i & 3)) place += key_at[own * 4 + part] == key;
 #pragma unroll
-    for (int r = 0; r < SMALL_ROUNDS; ++r) {
-        const int i = first + r * 64;
-        if (i < n) {
-            keys[i] = key[r];
-            order[i] = from[r];
-            if (rows)
-                rows[i] = max(bag_of(bounds, kind, fixed, bags, from[r], 0, bags), 0);
-        }
+    for (int d = 8; d; d >>= 1) place += __shfl_xor(place, d, 16);
+    if (part == 0) {
+        keys[place] = key;
+        order[place] = i;
+        if (rows) rows[place] = row;
     }
 }
 
@@ -381,6 +443,27 @@ int digit_passes(int V, int& bits) {
     return passes;
 }
 
+template <int ROUNDS>
+void sort_by_digits(Source src, const Bags& bags, int* keys, int* order,
+                    int* rows, int* work, hipStream_t stream) {
+    int bits;
+    const int passes = digit_passes(src.V, bits);
+    const int n = src.n, tiles = ks_ceil_div(n, ROUNDS * 256);
+    int2* pairs[2] = {(int2*)work, (int2*)(work + 2ll * n)};
+    int* totals = work + 4ll * n;
+    int* counts = totals + (1 << bits);
+    src.bag = rows ? counts + (long long)tiles * (1 << bits) : nullptr;
+    for (int p = 0; p < passes; ++p) {
+        int2* to = p == passes - 1 ? nullptr : pairs[p & 1];
+        digit_count_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
+            src, p * bits, bits, counts, tiles, bags);
+        digit_scan_kernel<<<1 << bits, 256, 0, stream>>>(counts, tiles, totals);
+        digit_move_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
+            src, p * bits, bits, counts, tiles, totals, to, keys, order, rows);
+        src.pairs = to;
+    }
+}
+
 }  // namespace
 
 // How many ints of workspace ks_token_sort needs.
@@ -388,7 +471,7 @@ KS_EXPORT long long ks_token_sort_work(int n, int V) {
     if (n <= SMALL) return 0;
     int bits;
     digit_passes(V, bits);
-    const long long tiles = ks_ceil_div(n, TILE);
+    const long long tiles = ks_ceil_div(n, rounds_of(n) * 256);
     return 5ll * n + (tiles + 1) * (1 << bits);
 }
 
@@ -398,34 +481,17 @@ KS_EXPORT int ks_token_sort(const void* ids, int ids_wide, int n, int V,
                             int kind, const void* bounds, int fixed, int bags,
                             int* keys, int* order, int* rows, int* starts,
                             int* work, hipStream_t stream) {
-    int bits;
-    const int passes = digit_passes(V, bits);
+    const Bags segments{bounds, kind, fixed, bags};
     if (n > 0 && n <= SMALL) {
-        // four waves have less to count and scan than sixteen: 777 tokens
-        // take 12.2 us against 14.1 us, starts included
-        auto* kernel = n <= SMALL / 4 ? small_sort_kernel<4> : small_sort_kernel<16>;
-        kernel<<<1, n <= SMALL / 4 ? 256 : 1024, 0, stream>>>(
-            ids, ids_wide, n, V, bounds, kind, fixed, bags, bits, passes, keys,
-            order, rows);
-    } else if (n > 0) {
-        const int tiles = ks_ceil_div(n, TILE);
-        int2* pairs[2] = {(int2*)work, (int2*)(work + 2ll * n)};
-        int* totals = work + 4ll * n;
-        int* counts = totals + (1 << bits);
-        int* bag = rows ? counts + (long long)tiles * (1 << bits) : nullptr;
-        if (bag)
-            position_bags_kernel<<<tiles, 256, 0, stream>>>(
-                bounds, kind, fixed, bags, n, bag);
-        Source src{nullptr, ids, ids_wide, n, V, bag};
-        for (int p = 0; p < passes; ++p) {
-            int2* to = p == passes - 1 ? nullptr : pairs[p & 1];
-            digit_count_kernel<<<tiles, 256, 0, stream>>>(src, p * bits, bits,
-                                                          counts, tiles);
-            digit_scan_kernel<<<1 << bits, 256, 0, stream>>>(counts, tiles, totals);
-            digit_move_kernel<<<tiles, 256, 0, stream>>>(
-                src, p * bits, bits, counts, tiles, totals, to, keys, order, rows);
-            src.pairs = to;
-        }
+        const int placing = ks_ceil_div(n, PLACED);
+        small_sort_kernel<<<placing + V / STARTS + 1, 256, 0, stream>>>(
+            ids, ids_wide, n, V, segments, keys, order, rows, starts, placing);
+        return (int)hipGetLastError();
+    }
+    if (n > 0) {
+        auto* sort = rounds_of(n) == FEW ? sort_by_digits<FEW> : sort_by_digits<MANY>;
+        sort(Source{nullptr, ids, ids_wide, n, V, nullptr}, segments, keys,
+             order, rows, work, stream);
     }
     token_starts_kernel<<<V / 256 + 1, 256, 0, stream>>>(keys, n, V, starts);
     return (int)hipGetLastError();

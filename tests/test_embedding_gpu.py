@@ -162,7 +162,8 @@ def test_ids_outside_every_bag_are_left_out(hip):
 
 @pytest.mark.parametrize("n,V", [
     (n, V) for V in (0, 1, 2, 255, 511, 512, 5000, 300000)
-    for n in (0, 1, 63, 4095, 4097, 20011)] + [(4097, 2 ** 27)])
+    for n in (0, 1, 63, 4095, 4097, 20011)] + [(4097, 2 ** 27),
+                                               (9001, 2 ** 27)])
 def test_plan_is_a_stable_sort(hip, n, V):
     g = gen(n + V)
     ids = some_ids(n, V, g, wide=n % 2 == 0)
@@ -173,6 +174,49 @@ def test_plan_is_a_stable_sort(hip, n, V):
     assert torch.equal(p.order.cpu().long(), order)
     starts = torch.searchsorted(want, torch.arange(V + 1))
     assert torch.equal(p.starts.cpu().long(), starts)
+
+
+@pytest.mark.parametrize("V", [1, 2047, 2048, 100001])
+@pytest.mark.parametrize("n", [17, 4000, 8191, 8192, 8193, 70001, 262144,
+                               262145, 400001])
+@pytest.mark.parametrize("bags", ["most of them empty", "long", "one", "ten",
+                                  "all empty", "fixed"])
+def test_plan_of_bags(hip, n, V, bags):
+    g = gen(n + V)
+    ids = some_ids(n, V, g, wide=n % 2 == 0)
+    if bags == "fixed":
+        n -= n % 3
+        ids = ids[:n].view(-1, 3)
+        p = hip.embedding_plan(ids, V, pooled=True)
+        bag, ids = torch.arange(n) // 3, ids.reshape(-1)
+    else:
+        # the first and the last few ids are in no bag
+        lo, hi = 3, n - 5
+        count = {"most of them empty": 3 * n, "long": 7, "one": 1,
+                 "ten": n // 10, "all empty": 1000}[bags]
+        at = torch.randint(lo, hi + 1, (count + 1,), generator=g).sort()[0]
+        if bags == "all empty":
+            at[:] = n // 2
+        else:
+            at[0], at[-1] = lo, hi
+        if bags == "most of them empty":
+            at[count // 3:2 * count // 3] = at[count // 3].clone()
+            at = at.sort()[0]
+        offsets = (at if n % 2 else at.int()).cuda()
+        p = hip.embedding_plan(ids, V, offsets)
+        i = torch.arange(n)
+        bag = torch.searchsorted(at, i, right=True) - 1
+        bag = torch.where((i < at[0]) | (i >= at[-1]), -1, bag)
+    ids = ids.cpu().long()
+    key = torch.where((ids >= 0) & (ids < V) & (bag >= 0), ids, V)
+    want, order = torch.sort(key, stable=True)
+    assert torch.equal(p.keys.cpu().long(), want)
+    assert torch.equal(p.order.cpu().long(), order)
+    assert torch.equal(p.starts.cpu().long(),
+                       torch.searchsorted(want, torch.arange(V + 1)))
+    there, rows = want < V, p.rows.cpu().long()
+    assert torch.equal(rows[there], bag[order][there])
+    assert rows.min() >= 0 and rows.max() < p.num_bags
 
 
 @pytest.mark.parametrize("src", TYPES)
