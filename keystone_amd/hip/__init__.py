@@ -233,7 +233,7 @@ def _launch(name: str, device: torch.device, *args) -> None:
     not, and on its current stream, which goes last."""
     fn = getattr(_lib, name)
     at = device.index
-    if at == torch.cuda.current_device():
+    if at == torch._C._cuda_getDevice():
         # the handle alone: a Stream object costs more than the launch
         code = fn(*args, torch._C._cuda_getCurrentRawStream(at))
     else:

@@ -106,7 +106,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     table = _matrix(table, "embedding_lookup.table")
     ids = _whole(ids, "embedding_lookup.ids", table.device)
     V, D = table.shape
-    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
+    out = table.new_empty((*ids.shape, D))
     n = ids.numel()
     if n and D:
         _launch("ks_embedding_lookup", table.device, ids.data_ptr(),

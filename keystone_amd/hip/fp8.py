@@ -160,16 +160,17 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
             raise ValueError(f"fp8_linear.bias: expected shape ({W.N},), got "
                              f"{tuple(bias.shape)}")
         bias = bias.contiguous()
-    out = torch.empty(M, W.N, dtype=X.dtype, device=X.device)
+    out = X.new_empty((M, W.N))
     if M == 0 or W.N == 0:
         return out
     if K == 0:
         return out.zero_() if bias is None else out.copy_(bias.expand(M, -1))
     kind = _TYPES[X.dtype]
-    work = torch.empty(lib.ks_fp8_work(kind, M, K, W.N), dtype=torch.uint8,
-                       device=X.device)
+    need = lib.ks_fp8_work(kind, M, K, W.N)
+    work = torch.empty(need, dtype=torch.uint8, device=X.device) \
+        if need else None
     _launch("ks_fp8_linear", X.device, X.data_ptr(), kind,
             X.stride(0) if M > 1 else K, W.data.data_ptr(),
             W.scales.data_ptr(), _ptr(bias), out.data_ptr(), M, K, W.N,
-            work.data_ptr())
+            _ptr(work))
     return out

@@ -21,7 +21,9 @@
 //     unit 59 % busy
 //   8192 x 65536 x 1000 f32: 845 us, 1.27 PFLOP/s (a large bfloat16 library
 //     product: 1.20)
-//   1 x 16384 x 1000 f32: 7.4 us, 2.3 TB/s of W from 63 blocks
+//   1 x 16384 x 1000 f32: 7.9 us, 2.1 TB/s of W from 63 blocks
+//   1021 x 8192 x 147 f32: 15.6 us with the join, X at 2.1 TB/s
+//   8192 x 8192 x 10 f32: 52 us, X at 5.2 TB/s
 #include "common.h"
 
 #include <cstdint>
@@ -57,43 +59,62 @@ __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
     }
 }
 
-// A lane's 32 elements of one block (row's pitch ld, K left from `k`): their
-// bytes, and 127 + the exponent.  The four lanes of a row, 16 apart, share it.
-template <typename T>
-__device__ __forceinline__ int quantise_block(const T* row, int k, int K, int g,
-                                              bool live, uint32_t (&w)[8]) {
-    float v[4][8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int at = k + j * 32 + g * 8;
-        load8(row + at, live ? K - at : 0, v[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
-    }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+// The exponent e of a block whose largest magnitude has the bits `top`.
+struct Scale {
+    int e;
+    float inv;      // 2^-e
+    bool bad;       // an infinity or a NaN: the block is NaN throughout
+};
+
+__device__ __forceinline__ Scale scale_of(uint32_t top) {
     // top = m 2^p with m in [1, 2); 448 = 1.75 2^8
     int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u);
     const bool bad = top >= 0x7f800000u;
     if (top == 0 || bad) e = 0;
     if (e < -117) e = -117;
-    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+    return {e, __uint_as_float((uint32_t)(127 - e) << 23), bad};
+}
+
+__device__ __forceinline__ uint32_t magnitude(const float (&v)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    return top;
+}
+
+__device__ __forceinline__ uint32_t four_bytes(const float* v, const Scale& s) {
+    int d = 0;
+    d = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * s.inv, v[1] * s.inv, d, false);
+    d = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * s.inv, v[3] * s.inv, d, true);
+    return s.bad ? 0x7f7f7f7fu : (uint32_t)d;
+}
+
+// A lane's 32 elements of one block, K of its row left from `left`, and their
+// bytes and 127 + the exponent.  The four lanes of a row, 16 apart, share it.
+template <typename T>
+__device__ __forceinline__ void load_block(const T* block, int left, int g,
+                                           bool live, float (&v)[4][8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            int d = 0;
-            d = __builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * h] * inv,
-                                                v[j][4 * h + 1] * inv, d, false);
-            d = __builtin_amdgcn_cvt_pk_fp8_f32(v[j][4 * h + 2] * inv,
-                                                v[j][4 * h + 3] * inv, d, true);
-            // a block that holds an infinity or a NaN is NaN throughout
-            w[2 * j + h] = bad ? 0x7f7f7f7fu : (uint32_t)d;
-        }
+        const int at = j * 32 + g * 8;
+        load8(block + at, live ? left - at : 0, v[j]);
     }
-    return 127 + e;
+}
+
+__device__ __forceinline__ int quantise_block(const float (&v)[4][8],
+                                              uint32_t (&w)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, magnitude(v[j]));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const Scale s = scale_of(top);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[2 * j + h] = four_bytes(v[j] + 4 * h, s);
+    return 127 + s.e;
 }
 
 // One wave a chunk: 16 rows by 128 of K.  scales[tile][K/512][16] has a
@@ -109,9 +130,11 @@ void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
     const int kb = (int)(chunk % kblocks), tile = (int)(chunk / kblocks);
     const int lane = threadIdx.x & 63;
     const int row = tile * 16 + (lane & 15);
+    float v[4][8];
     uint32_t w[8];
-    const int e = quantise_block(x + (long long)row * ld, kb * 128, K, lane >> 4,
-                                 row < rows, w);
+    load_block(x + (long long)row * ld + kb * 128, K - kb * 128, lane >> 4,
+               row < rows, v);
+    const int e = quantise_block(v, w);
     unsigned char* to = q + chunk * CHUNK + lane * 16;
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(to + 1024) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -242,8 +265,8 @@ __device__ __forceinline__ int scale_at(const unsigned* scales, int kq, int tile
 }
 
 // A wave has TM x TN tiles of 16 x 16; its operands come straight from
-// memory.  Waves are counted along N first: neighbours share X's rows.  Split s of gridDim.y takes K blocks [s kper, (s + 1) kper); with
-// more than one split, `part` [splits][M][N] takes the sums.
+// memory.  Waves are counted along N first: neighbours share X's rows.  Split s
+// of gridDim.y takes K blocks [s kper, (s + 1) kper); with more than one split, `part` [splits][M][N] takes the sums.
 // EXACT: products and sums for 32-bit outputs.
 template <typename T, int TM, int TN, bool EXACT>
 __global__ __launch_bounds__(256)
@@ -280,21 +303,83 @@ void fp8_gemm_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
         m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N);
 }
 
+// X itself, for the kernels that quantise what they multiply.
+template <typename T>
+struct Rows {
+    const T* x;
+    long long ld;
+    int K;
+};
+
+// The waves' sums of a tile of 16 rows by TN of 16 columns are added up.
+template <typename T, int TN, int WAVES>
+__device__ __forceinline__ void add_waves(const f32x4 (&acc)[TN],
+                                          f32x4 (*sums)[TN][64], const Gemm& a,
+                                          int tile, int n0, T* y, float* part,
+                                          const float* bias) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TN * 64; i += WAVES * 64) {
+        const int j = i >> 6, l = i & 63;
+        f32x4 s = sums[0][j][l];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += sums[w][j][l];
+        const int m = tile * 16 + (l & 15), n = (n0 + j) * 16 + (l >> 4) * 4;
+        if (m >= a.M || n >= a.N) continue;
+        if (part)
+            store_columns<float>(part + (long long)blockIdx.y * a.M * a.N, a.N,
+                                 m, n, a.N, s);
+        else
+            store_columns<T>(y, a.N, m, n, a.N, s + bias_at(bias, n, a.N));
+    }
+}
+
 // Few rows, or few columns: a block has one tile of 16 rows by TN of 16
 // columns, its 16 waves share K (of split blockIdx.y) and add up in LDS.
-template <typename T, int TN>
+// STAGED: the block first quantises its rows into LDS, eight lanes for 128 of
+// K, 16 bytes a lane.
+constexpr int STAGE = 32768;
+
+template <typename T, int TN, bool STAGED>
 __global__ __launch_bounds__(1024)
-void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
-                     const float* __restrict__ bias, int kper) {
+void fp8_rows_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
+                     float* __restrict__ part, const float* __restrict__ bias,
+                     int kper) {
     constexpr bool EXACT = sizeof(T) == 4;
     __shared__ f32x4 sums[16][TN][64];
+    __shared__ uint4 staged[STAGED ? STAGE / 16 : 1];
+    __shared__ unsigned char exponents[STAGED ? STAGE / 128 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ntiles = ks_ceil_div(a.N, 16), groups = ks_ceil_div(ntiles, TN);
     const int tile = blockIdx.x / groups, n0 = blockIdx.x % groups * TN;
     const int kq = (a.kblocks + 3) / 4;
-    const int k1 = min(a.kblocks, ((int)blockIdx.y + 1) * kper);
+    const int k0 = blockIdx.y * kper, k1 = min(a.kblocks, k0 + kper);
+    const int rows = min(16, a.M - tile * 16);
+    if constexpr (STAGED) {
+        const int p = threadIdx.x >> 2 & 1, g = threadIdx.x & 3;
+        for (int u = threadIdx.x >> 3; u < rows * (k1 - k0); u += 128) {
+            const int kb = k0 + u / rows, m = u % rows;
+            const int at = kb * 128 + p * 64 + g * 8;
+            const T* x = src.x + (long long)(tile * 16 + m) * src.ld + at;
+            float v[2][8];
+            load8(x, src.K - at, v[0]);
+            load8(x + 32, src.K - at - 32, v[1]);
+            uint32_t top = max(magnitude(v[0]), magnitude(v[1]));
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1)
+                top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+            const Scale s = scale_of(top);
+            staged[u * 8 + (threadIdx.x & 7)] =
+                make_uint4(four_bytes(v[0], s), four_bytes(v[0] + 4, s),
+                           four_bytes(v[1], s), four_bytes(v[1] + 4, s));
+            if ((threadIdx.x & 7) == 0) exponents[u] = (unsigned char)(127 + s.e);
+        }
+        __syncthreads();
+    }
     f32x4 acc[1][TN] = {};
-    for (int kb = blockIdx.y * kper + wave; kb < k1; kb += 16) {
+    for (int kb = k0 + wave; kb < k1; kb += 16) {
         i32x8 xf[1], wf[TN];
         int xs[1], ws[TN];
 #pragma unroll
@@ -303,25 +388,83 @@ void fp8_rows_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
             wf[j] = load_chunk(a.wq + ((long long)t * a.kblocks + kb) * CHUNK, lane);
             ws[j] = scale_at(a.ws, kq, t, kb, lane);
         }
-        xf[0] = load_chunk(a.xq + ((long long)tile * a.kblocks + kb) * CHUNK, lane);
-        xs[0] = scale_at(a.xs, kq, tile, kb, lane);
+        if constexpr (STAGED) {
+            const int m = lane & 15;
+            xf[0] = i32x8{};
+            xs[0] = 127;
+            if (m < rows) {
+                const int u = (kb - k0) * rows + m;
+                const uint4 lo = staged[u * 8 + (lane >> 4)];
+                const uint4 hi = staged[u * 8 + 4 + (lane >> 4)];
+                xf[0] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w,
+                              (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+                xs[0] = exponents[u];
+            }
+        } else {
+            xf[0] = load_chunk(a.xq + ((long long)tile * a.kblocks + kb) * CHUNK,
+                               lane);
+            xs[0] = scale_at(a.xs, kq, tile, kb, lane);
+        }
         multiply<EXACT, 1, TN>(xf, xs, wf, ws, acc);
     }
+    add_waves<T, TN, 16>(acc[0], sums, a, tile, n0, y, part, bias);
+}
+
+// Few columns: a block has TM tiles of 16 rows by all of them, its eight waves
+// share K, and a wave quantises the rows that it multiplies, so that X is read
+// once and never written back.
+template <typename T, int TM, int TN>
+__global__ __launch_bounds__(512, TM * TN > 5 ? 2 : 4)
+void fp8_narrow_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
+                       float* __restrict__ part, const float* __restrict__ bias,
+                       int kper) {
+    constexpr bool EXACT = sizeof(T) == 4;
+    __shared__ f32x4 sums[8][TN][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int ntiles = ks_ceil_div(a.N, 16), tile = blockIdx.x * TM;
+    const int kq = (a.kblocks + 3) / 4;
+    const int k1 = min(a.kblocks, ((int)blockIdx.y + 1) * kper);
+    const int row = tile * 16 + (lane & 15);
+    const T* const x = src.x + (long long)row * src.ld;
+    float v[TM][4][8];
+    const auto load_rows = [&](int kb) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[0][j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < TN * 64; i += 1024) {
-        const int j = i >> 6, l = i & 63;
-        f32x4 s = sums[0][j][l];
+        for (int i = 0; i < TM; ++i)
+            load_block(x + i * 16 * src.ld + kb * 128, src.K - kb * 128,
+                       lane >> 4, row + i * 16 < a.M && kb < k1, v[i]);
+    };
+    int kb = blockIdx.y * kper + wave;
+    load_rows(kb);
+    f32x4 acc[TM][TN] = {};
+    for (; kb < k1; kb += 8) {
+        i32x8 xf[TM];
+        int xs[TM];
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s += sums[w][j][l];
-        const int m = tile * 16 + (l & 15), n = (n0 + j) * 16 + (l >> 4) * 4;
-        if (m >= a.M || n >= a.N) continue;
-        if (part)
-            store_columns<float>(part + (long long)blockIdx.y * a.M * a.N, a.N,
-                                 m, n, a.N, s);
-        else
-            store_columns<T>(y, a.N, m, n, a.N, s + bias_at(bias, n, a.N));
+        for (int i = 0; i < TM; ++i) {
+            uint32_t w[8];
+            xs[i] = quantise_block(v[i], w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) xf[i][k] = (int)w[k];
+        }
+        load_rows(kb + 8);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int t = min(j, ntiles - 1);
+            const i32x8 wf[1] = {
+                load_chunk(a.wq + ((long long)t * a.kblocks + kb) * CHUNK, lane)};
+            const int ws[1] = {scale_at(a.ws, kq, t, kb, lane)};
+            f32x4 column[TM][1];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) column[i][0] = acc[i][j];
+            multiply<EXACT, TM, 1>(xf, xs, wf, ws, column);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) acc[i][j] = column[i][0];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        if (i) __syncthreads();
+        add_waves<T, TN, 8>(acc[i], sums, a, tile + i, 0, y, part, bias);
     }
 }
 
@@ -566,13 +709,50 @@ int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
     return (int)hipGetLastError();
 }
 
+// Splits begin at whole words of scales.
+int per_split(int kblocks, int splits) {
+    return ks_ceil_div(ks_ceil_div(kblocks, splits), 4) * 4;
+}
+
+int rows_splits(int M, int N, int kblocks) {
+    // 65 MB of W take 27 us from 63 blocks, and 17 us from 252 and a join;
+    // 16 MB take 7.4 us and gain nothing
+    long long s = 256 / ((long long)ks_ceil_div(M, 16) * ks_ceil_div(N, 16));
+    if (s > kblocks / 128) s = kblocks / 128;
+    return s < 1 || kblocks < 256 ? 1 : (int)s;
+}
+
+int rows_per(int M, int N, int kblocks) {
+    return per_split(kblocks, rows_splits(M, N, kblocks));
+}
+
+constexpr int MOST_NARROW = 10;
+
+// Tiles of rows in a block of fp8_narrow_kernel: two read W half as often, where
+// that leaves a block for each compute unit.  8192 x 8192 x 147 bf16: 60 us,
+// 76 us with one; 4096 rows: 57 and 40 us.  32-bit results with two gain 5 us at
+// 147 columns and lose 4 us at 100.
+template <typename T>
+int narrow_down(int M, int nt) {
+    return sizeof(T) == 2 && nt > 5 && ks_ceil_div(M, 32) >= 256 ? 2 : 1;
+}
+
 // Which kernel a product goes through.
-enum Kind { ROWS, TILES, LARGE };
+enum Kind { STAGED, NARROW, ROWS, TILES, LARGE };
 
 Kind kind_of(int type, int M, int N, int kblocks) {
     const int mt = ks_ceil_div(M, 16), nt = ks_ceil_div(N, 16);
-    if (mt == 1 || (long long)mt * nt <= 512 || (mt <= 64 && nt <= 16))
-        return ROWS;
+    const bool few = mt == 1 || (long long)mt * nt <= 512 || (mt <= 64 && nt <= 16);
+    // 1 x 16384 x 1000 f32: 7.9 us staged, 10.9 us with a launch for X; 128 x
+    // 2048 x 1000 7.9 and 7.5 us, but 9.2 and 12 us with the host's part.  1021 x
+    // 2048 x 147 7.4 us, 10.6 us by NARROW; 2048 rows 17.5 and 11 us.
+    if (few && (long long)(M < 16 ? M : 16) * rows_per(M, N, kblocks) * 128 <= STAGE)
+        return STAGED;
+    // 1021 x 8192 x 147 f32: 15.6 us, 18.6 us by ROWS; 8192 x 65536 x 20 bf16: 257
+    // us, 420 us by TILES; 512 x 4096 x 147 f32: 12.5 us, 10.8 us by ROWS
+    if (nt <= MOST_NARROW && mt >= 64) return NARROW;
+    // 1000 x 8192 x 250 f32: 25 us, 27 us by TILES
+    if (few) return ROWS;
     // At least four steps for each compute unit, eight of the longer ones for
     // 32-bit results.  bf16: 2048 x 2048 x 2048 has four, 37 us against 38 us by
     // TILES; 8192 x 1024 x 2000 eight, 39 against 53; 1024 x 4096 x 1000 two,
@@ -595,12 +775,11 @@ int tiles_down(int M, int N) {
 // How many ways K is split: enough blocks to fill the card.
 int splits_of(int type, int M, int N, int kblocks) {
     const Kind kind = kind_of(type, M, N, kblocks);
-    if (kind == ROWS) {
-        // 65 MB of W take 27 us from 63 blocks, and 17 us from 252 and a join;
-        // 16 MB take 7.4 us and gain nothing
-        long long s = 256 / ((long long)ks_ceil_div(M, 16) * ks_ceil_div(N, 16));
-        if (s > kblocks / 128) s = kblocks / 128;
-        return s < 1 || kblocks < 256 ? 1 : (int)s;
+    if (kind == ROWS || kind == STAGED) return rows_splits(M, N, kblocks);
+    if (kind == NARROW) {
+        long long s = 256 / ks_ceil_div(M, 16);
+        if (s > kblocks / 16) s = kblocks / 16;
+        return s < 1 ? 1 : (int)s;
     }
     if (kind == LARGE) {
         const long long blocks = (long long)ks_ceil_div(M, BIG) * ks_ceil_div(N, BIG);
@@ -616,29 +795,48 @@ int splits_of(int type, int M, int N, int kblocks) {
 }
 
 template <typename T>
-void rows(const Gemm& a, T* y, float* part, const float* bias,
-          int splits, int kper, hipStream_t stream) {
+void rows(const Gemm& a, const Rows<T>& src, bool staged, T* y, float* part,
+          const float* bias, int splits, int kper, hipStream_t stream) {
     const int nt = ks_ceil_div(a.N, 16), mt = ks_ceil_div(a.M, 16);
-    // 1021 x 8192 x 147: 12 us with three columns of tiles a block in 32 bits
-    // (15 with five, whose widening takes longer), with five in 16 (13 with
-    // three)
+    // 900 x 4096 x 147 f32: 13.5 us with three columns of tiles a block, 13.9 us
+    // with four; 1000 x 8192 x 250 bf16: 21 us with five, 23 us with three
     constexpr int WIDE = sizeof(T) == 4 ? 3 : 5;
     const int tn = (long long)mt * nt <= 512 ? 1 : WIDE;
     const unsigned grid = (unsigned)mt * ks_ceil_div(nt, tn);
-    auto* kernel = tn == 1 ? fp8_rows_kernel<T, 1> : fp8_rows_kernel<T, WIDE>;
-    kernel<<<dim3(grid, splits), 1024, 0, stream>>>(a, y, part, bias, kper);
+    auto* kernel =
+        staged ? tn == 1 ? fp8_rows_kernel<T, 1, true> : fp8_rows_kernel<T, WIDE, true>
+               : tn == 1 ? fp8_rows_kernel<T, 1, false>
+                         : fp8_rows_kernel<T, WIDE, false>;
+    kernel<<<dim3(grid, splits), 1024, 0, stream>>>(a, src, y, part, bias, kper);
 }
 
 template <typename T>
-int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
-         hipStream_t stream) {
+void narrow(const Gemm& a, const Rows<T>& src, T* y, float* part,
+            const float* bias, int splits, int kper, hipStream_t stream) {
+    const int nt = ks_ceil_div(a.N, 16);
+    const int down = narrow_down<T>(a.M, nt);
+    auto* kernel = fp8_narrow_kernel<T, 1, MOST_NARROW>;
+    if (nt <= 5)
+        kernel = nt == 1   ? fp8_narrow_kernel<T, 1, 1>
+                 : nt == 2 ? fp8_narrow_kernel<T, 1, 2>
+                           : fp8_narrow_kernel<T, 1, 5>;
+    if constexpr (sizeof(T) == 2)
+        if (down == 2) kernel = fp8_narrow_kernel<T, 2, MOST_NARROW>;
+    kernel<<<dim3(ks_ceil_div(a.M, 16 * down), splits), 512, 0, stream>>>(
+        a, src, y, part, bias, kper);
+}
+
+template <typename T>
+int gemm(const Gemm& a, const Rows<T>& src, void* y, float* part,
+         const float* bias, int type, hipStream_t stream) {
     const Kind kind = kind_of(type, a.M, a.N, a.kblocks);
     const int splits = splits_of(type, a.M, a.N, a.kblocks);
-    // splits begin at whole words of scales
-    const int kper = ks_ceil_div(ks_ceil_div(a.kblocks, splits), 4) * 4;
+    const int kper = per_split(a.kblocks, splits);
     float* parts = splits > 1 ? part : nullptr;
-    if (kind == ROWS) {
-        rows<T>(a, (T*)y, parts, bias, splits, kper, stream);
+    if (kind == ROWS || kind == STAGED) {
+        rows<T>(a, src, kind == STAGED, (T*)y, parts, bias, splits, kper, stream);
+    } else if (kind == NARROW) {
+        narrow<T>(a, src, (T*)y, parts, bias, splits, kper, stream);
     } else if (kind == LARGE) {
         const int mb = ks_ceil_div(a.M, BIG), nb = ks_ceil_div(a.N, BIG);
         fp8_gemm_big_kernel<T><<<mb * nb * splits, 256, 0, stream>>>(
@@ -662,17 +860,27 @@ int gemm(const Gemm& a, void* y, float* part, const float* bias, int type,
     return (int)hipGetLastError();
 }
 
+template <typename T>
+int linear(const Gemm& a, const void* x, long long ld, int K, void* y, float* part,
+           const float* bias, int type, hipStream_t stream) {
+    return gemm<T>(a, Rows<T>{(const T*)x, ld, K}, y, part, bias, type, stream);
+}
+
 // Where a call's workspace has what.
 struct Work {
+    bool quantised;    // before the product, in a launch of its own
     long long scales, part, bytes;
 };
 
 Work work_of(int type, int M, int K, int N) {
     const long long tiles = ks_ceil_div(M, 16), kb = ks_ceil_div(K, 128);
     const int splits = splits_of(type, M, N, (int)kb);
+    const Kind kind = kind_of(type, M, N, (int)kb);
     Work w;
-    w.scales = tiles * kb * CHUNK;
-    w.part = (w.scales + tiles * ((kb + 3) / 4) * 64 + 255) / 256 * 256;
+    w.quantised = kind != STAGED && kind != NARROW;
+    w.scales = w.quantised ? tiles * kb * CHUNK : 0;
+    w.part = w.quantised
+                 ? (w.scales + tiles * ((kb + 3) / 4) * 64 + 255) / 256 * 256 : 0;
     w.bytes = w.part + (splits > 1 ? 4ll * splits * M * N : 0);
     return w;
 }
@@ -707,15 +915,18 @@ KS_EXPORT int ks_fp8_linear(const void* x, int type, long long ld,
                             unsigned char* work, hipStream_t stream) {
     if (M == 0 || N == 0) return 0;
     const Work w = work_of(type, M, K, N);
-    const int code = ks_fp8_quantise(x, type, ld, M, K, work, work + w.scales,
-                                     stream);
-    if (code) return code;
+    if (w.quantised) {
+        const int code = ks_fp8_quantise(x, type, ld, M, K, work,
+                                         work + w.scales, stream);
+        if (code) return code;
+    }
     const Gemm a{work, (const unsigned*)(work + w.scales), wq, ws, M, N,
                  ks_ceil_div(K, 128)};
     float* part = (float*)(work + w.part);
     switch (type) {
-        case 0: return gemm<float>(a, y, part, bias, type, stream);
-        case 1: return gemm<__bf16>(a, y, part, bias, type, stream);
-        default: return gemm<_Float16>(a, y, part, bias, type, stream);
+        case 0: return linear<float>(a, x, ld, K, y, part, bias, type, stream);
+        case 1: return linear<__bf16>(a, x, ld, K, y, part, bias, type, stream);
+        default:
+            return linear<_Float16>(a, x, ld, K, y, part, bias, type, stream);
     }
 }

@@ -98,7 +98,14 @@ def test_pack_at_the_borders(hip):
 @pytest.mark.parametrize("M,K,N", [
     (1, 1, 1), (1, 128, 16), (16, 128, 16), (17, 130, 19), (1, 16384, 1000),
     (5, 8192, 147), (64, 1000, 20), (65, 640, 257), (200, 4096, 130),
-    (300, 300, 300), (1021, 512, 2)])
+    (300, 300, 300), (1021, 512, 2),
+    # X quantised where it is multiplied: few rows, a few more, of long and of
+    # short K, split or not
+    (2, 16383, 33), (3, 10900, 40), (1, 70001, 1000), (16, 2048, 77),
+    (15, 2049, 50), (33, 2047, 161), (1024, 2048, 256), (1023, 1025, 147),
+    # few columns of many rows
+    (1009, 2049, 16), (1025, 3001, 17), (2500, 129, 33), (1500, 4200, 80),
+    (1021, 8192, 147), (1300, 5000, 160), (8170, 300, 147), (8165, 2500, 81)])
 def test_linear(hip, dtype, M, K, N):
     X, W, b = operands(M, K, N, dtype)
     packed = hip.fp8_pack(W)
@@ -123,6 +130,19 @@ def test_large_product(hip, dtype, M, K, N):
     rows = torch.arange(0, M, 7)
     rows = torch.cat([rows, torch.arange(M - 20, M)])
     check(hip, got[rows.cuda()], X[rows.cuda()], W, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(40, 700, 20), (1100, 2300, 90),
+                                   (8200, 190, 100)])
+def test_strided_and_misaligned_narrow(hip, dtype, M, K, N):
+    base = torch.randn(M + 3, K + 11, device="cuda").to(dtype)
+    base[:, K + 5:] = float("nan")
+    W = torch.randn(K, N, device="cuda")
+    packed = hip.fp8_pack(W)
+    for X in (base[1:M + 1, 5:K + 5], base[:M, 4:K + 4], base[1:2, :K].expand(M, K),
+              base[::2, 3:K + 3]):
+        check(hip, hip.fp8_linear(X, packed), X, W, None)
 
 
 def test_strided_and_misaligned_rows(hip):
@@ -157,8 +177,21 @@ def test_nan_and_infinity_stay_in_their_rows(hip):
     assert y.cpu()[~bad].eq(512).all()
 
 
-def test_captured_and_replayed(hip):
-    X, W, b = operands(9, 4096, 147, torch.float32)
+@pytest.mark.parametrize("M,K,N", [(1200, 700, 20), (1100, 9000, 147)])
+def test_nan_and_infinity_in_narrow_products(hip, M, K, N):
+    X = torch.ones(M, K, device="cuda")
+    X[3, 200], X[20, 7], X[M - 1, K - 1] = float("nan"), float("inf"), -float("inf")
+    y = hip.fp8_linear(X, hip.fp8_pack(torch.ones(K, N, device="cuda")))
+    bad = torch.zeros(M, dtype=torch.bool)
+    bad[[3, 20, M - 1]] = True
+    assert y.cpu()[bad].isnan().all()
+    assert y.cpu()[~bad].eq(K).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(9, 4096, 147), (9, 9000, 147), (1, 800, 20),
+                                   (1100, 9000, 147)])
+def test_captured_and_replayed(hip, M, K, N):
+    X, W, b = operands(M, K, N, torch.float32)
     packed = hip.fp8_pack(W)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
