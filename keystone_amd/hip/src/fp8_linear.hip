@@ -22,7 +22,7 @@
 //   8192 x 65536 x 1000 f32: 845 us, 1.27 PFLOP/s (a large bfloat16 library
 //     product: 1.20)
 //   1 x 16384 x 1000 f32: 7.9 us, 2.1 TB/s of W from 63 blocks
-//   1021 x 8192 x 147 f32: 15.6 us with the join, X at 2.1 TB/s
+//   1021 x 8192 x 147 f32: 15.4 us with the join, X at 2.2 TB/s
 //   8192 x 8192 x 10 f32: 52 us, X at 5.2 TB/s
 #include "common.h"
 
@@ -311,21 +311,33 @@ struct Rows {
     int K;
 };
 
-// The waves' sums of a tile of 16 rows by TN of 16 columns are added up.
-template <typename T, int TN, int WAVES>
-__device__ __forceinline__ void add_waves(const f32x4 (&acc)[TN],
-                                          f32x4 (*sums)[TN][64], const Gemm& a,
-                                          int tile, int n0, T* y, float* part,
-                                          const float* bias) {
+// The waves' sums of a tile of 16 rows by TN of 16 columns are added up.  Where
+// `sums` has room for half of the waves, the others add theirs to them first.
+template <typename T, int TN, int WAVES, int ROOM>
+__device__ __forceinline__ void add_waves(f32x4 (&acc)[TN], f32x4 (*sums)[TN][64],
+                                          const Gemm& a, int tile, int n0, T* y,
+                                          float* part, const float* bias) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (ROOM < WAVES) {
+        static_assert(WAVES == 2 * ROOM);
+        if (wave >= ROOM)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[j];
+            for (int j = 0; j < TN; ++j) sums[wave - ROOM][j][lane] = acc[j];
+        __syncthreads();
+        if (wave < ROOM)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[j] += sums[wave][j][lane];
+    }
+    // a wave writes where it has read itself
+    if (wave < ROOM)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[j];
     __syncthreads();
-    for (int i = threadIdx.x; i < TN * 64; i += WAVES * 64) {
+    for (int i = threadIdx.x; i < TN * 64; i += blockDim.x) {
         const int j = i >> 6, l = i & 63;
         f32x4 s = sums[0][j][l];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += sums[w][j][l];
+        for (int w = 1; w < ROOM; ++w) s += sums[w][j][l];
         const int m = tile * 16 + (l & 15), n = (n0 + j) * 16 + (l >> 4) * 4;
         if (m >= a.M || n >= a.N) continue;
         if (part)
@@ -407,18 +419,24 @@ void fp8_rows_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
         }
         multiply<EXACT, 1, TN>(xf, xs, wf, ws, acc);
     }
-    add_waves<T, TN, 16>(acc[0], sums, a, tile, n0, y, part, bias);
+    add_waves<T, TN, 16, 16>(acc[0], sums, a, tile, n0, y, part, bias);
 }
 
-// Few columns: a block has TM tiles of 16 rows by all of them, its eight waves
-// share K, and a wave quantises the rows that it multiplies, so that X is read
-// once and never written back.
+// Few columns: a block has TM tiles of 16 rows by all of them, its waves share K,
+// and a wave quantises the rows that it multiplies, so that X is read once and
+// never written back.  Sixteen waves hide each other's loads (1021 x 8192 x 147
+// bf16: 13.4 us, 15.1 us with eight that load ahead); two tiles leave registers
+// for eight, which load the next rows ahead.
+constexpr int narrow_waves(int down) { return down == 1 ? 16 : 8; }
+
 template <typename T, int TM, int TN>
-__global__ __launch_bounds__(512, TM * TN > 5 ? 2 : 4)
+__global__ __launch_bounds__(64 * narrow_waves(TM))
 void fp8_narrow_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
                        float* __restrict__ part, const float* __restrict__ bias,
                        int kper) {
     constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int WAVES = narrow_waves(TM);
+    constexpr bool AHEAD = WAVES == 8;
     __shared__ f32x4 sums[8][TN][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ntiles = ks_ceil_div(a.N, 16), tile = blockIdx.x * TM;
@@ -434,9 +452,10 @@ void fp8_narrow_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
                        lane >> 4, row + i * 16 < a.M && kb < k1, v[i]);
     };
     int kb = blockIdx.y * kper + wave;
-    load_rows(kb);
+    if (AHEAD) load_rows(kb);
     f32x4 acc[TM][TN] = {};
-    for (; kb < k1; kb += 8) {
+    for (; kb < k1; kb += WAVES) {
+        if (!AHEAD) load_rows(kb);
         i32x8 xf[TM];
         int xs[TM];
 #pragma unroll
@@ -446,7 +465,7 @@ void fp8_narrow_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
 #pragma unroll
             for (int k = 0; k < 8; ++k) xf[i][k] = (int)w[k];
         }
-        load_rows(kb + 8);
+        if (AHEAD) load_rows(kb + WAVES);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             const int t = min(j, ntiles - 1);
@@ -464,7 +483,7 @@ void fp8_narrow_kernel(Gemm a, Rows<T> src, T* __restrict__ y,
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         if (i) __syncthreads();
-        add_waves<T, TN, 8>(acc[i], sums, a, tile + i, 0, y, part, bias);
+        add_waves<T, TN, WAVES, 8>(acc[i], sums, a, tile + i, 0, y, part, bias);
     }
 }
 
@@ -729,12 +748,14 @@ int rows_per(int M, int N, int kblocks) {
 constexpr int MOST_NARROW = 10;
 
 // Tiles of rows in a block of fp8_narrow_kernel: two read W half as often, where
-// that leaves a block for each compute unit.  8192 x 8192 x 147 bf16: 60 us,
-// 76 us with one; 4096 rows: 57 and 40 us.  32-bit results with two gain 5 us at
-// 147 columns and lose 4 us at 100.
-template <typename T>
-int narrow_down(int M, int nt) {
-    return sizeof(T) == 2 && nt > 5 && ks_ceil_div(M, 32) >= 256 ? 2 : 1;
+// that leaves work for each compute unit.  bf16, one tile and two: 8192 x 8192 x
+// 147 76 and 60 us, 4096 x 8192 x 147 40 and 37 us, 2048 x 2048 x 147 9.5 and 14
+// us.  32-bit results with two gain 5 us of 77 at 8192 x 8192 x 147 and lose 4 of
+// 41 at 100 columns.
+int narrow_down(int type, int M, int nt, int kblocks) {
+    const long long blocks = ks_ceil_div(M, 32);
+    return type != 0 && nt > 5 && (blocks >= 256 || blocks * kblocks >= 8192)
+               ? 2 : 1;
 }
 
 // Which kernel a product goes through.
@@ -748,7 +769,7 @@ Kind kind_of(int type, int M, int N, int kblocks) {
     // 2048 x 147 7.4 us, 10.6 us by NARROW; 2048 rows 17.5 and 11 us.
     if (few && (long long)(M < 16 ? M : 16) * rows_per(M, N, kblocks) * 128 <= STAGE)
         return STAGED;
-    // 1021 x 8192 x 147 f32: 15.6 us, 18.6 us by ROWS; 8192 x 65536 x 20 bf16: 257
+    // 1021 x 8192 x 147 f32: 15.4 us, 18.6 us by ROWS; 8192 x 65536 x 20 bf16: 250
     // us, 420 us by TILES; 512 x 4096 x 147 f32: 12.5 us, 10.8 us by ROWS
     if (nt <= MOST_NARROW && mt >= 64) return NARROW;
     // 1000 x 8192 x 250 f32: 25 us, 27 us by TILES
@@ -777,7 +798,8 @@ int splits_of(int type, int M, int N, int kblocks) {
     const Kind kind = kind_of(type, M, N, kblocks);
     if (kind == ROWS || kind == STAGED) return rows_splits(M, N, kblocks);
     if (kind == NARROW) {
-        long long s = 256 / ks_ceil_div(M, 16);
+        const int nt = ks_ceil_div(N, 16);
+        long long s = 256 / ks_ceil_div(M, 16 * narrow_down(type, M, nt, kblocks));
         if (s > kblocks / 16) s = kblocks / 16;
         return s < 1 ? 1 : (int)s;
     }
@@ -814,7 +836,7 @@ template <typename T>
 void narrow(const Gemm& a, const Rows<T>& src, T* y, float* part,
             const float* bias, int splits, int kper, hipStream_t stream) {
     const int nt = ks_ceil_div(a.N, 16);
-    const int down = narrow_down<T>(a.M, nt);
+    const int down = narrow_down(sizeof(T) == 4 ? 0 : 1, a.M, nt, a.kblocks);
     auto* kernel = fp8_narrow_kernel<T, 1, MOST_NARROW>;
     if (nt <= 5)
         kernel = nt == 1   ? fp8_narrow_kernel<T, 1, 1>
@@ -822,8 +844,8 @@ void narrow(const Gemm& a, const Rows<T>& src, T* y, float* part,
                            : fp8_narrow_kernel<T, 1, 5>;
     if constexpr (sizeof(T) == 2)
         if (down == 2) kernel = fp8_narrow_kernel<T, 2, MOST_NARROW>;
-    kernel<<<dim3(ks_ceil_div(a.M, 16 * down), splits), 512, 0, stream>>>(
-        a, src, y, part, bias, kper);
+    kernel<<<dim3(ks_ceil_div(a.M, 16 * down), splits), 64 * narrow_waves(down), 0,
+             stream>>>(a, src, y, part, bias, kper);
 }
 
 template <typename T>
