@@ -679,9 +679,10 @@ int lanes_log(int D, int vec) {
     if (cols > 64 && (cols + 31) / 32 * 5 <= (cols + 63) / 64 * 8) return 5;
     return log2_up(cols, 6);
 }
-// A gradient of up to 1024 tokens has none: the calls for 777 of 100 f32 take
-// 20.8 us without the join's launch and 25.7 us with it.  Where all 1024 are one
-// token, of 512 f32, its block takes 24 us alone, against 14 us.
+// A gradient of up to 1024 tokens has none: 777 of 100 f32 take 11.1 us, sort
+// included, without the join's launch and 12.4 us with it, and the host's part
+// of a launch goes too.  Where all 1024 are one token, of 512 f32, its block
+// takes 25 us alone, against 14 us.
 int chunk_of(int D, int vec, int n, bool sorted) {
     if (sorted && n <= 1024) return 1024;
     const int c = 8192 >> lanes_log(D, vec);

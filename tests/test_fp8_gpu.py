@@ -105,7 +105,8 @@ def test_pack_at_the_borders(hip):
     (15, 2049, 50), (33, 2047, 161), (1024, 2048, 256), (1023, 1025, 147),
     # few columns of many rows
     (1009, 2049, 16), (1025, 3001, 17), (2500, 129, 33), (1500, 4200, 80),
-    (1021, 8192, 147), (1300, 5000, 160), (8170, 300, 147), (8165, 2500, 81)])
+    (1021, 8192, 147), (1300, 5000, 160), (8170, 300, 147), (8165, 2500, 81),
+    (2100, 16700, 150)])
 def test_linear(hip, dtype, M, K, N):
     X, W, b = operands(M, K, N, dtype)
     packed = hip.fp8_pack(W)
