@@ -707,6 +707,7 @@ def sym_rectify(X: torch.Tensor, alpha: float = 0.0) -> torch.Tensor:
 
 
 from .counter_dropout import dropout, dropout_threshold  # noqa: E402
-from .embedding import (EmbeddingPlan, embedding_bag,  # noqa: E402
-                        embedding_grad, embedding_lookup, embedding_plan)
+from .embedding import (MAX_TOKENS, EmbeddingPlan,  # noqa: E402
+                        embedding_bag, embedding_grad, embedding_lookup,
+                        embedding_plan)
 from .fp8 import Fp8Weight, fp8_linear, fp8_pack, fp8_round  # noqa: E402

@@ -23,11 +23,11 @@ import torch
 from . import _launch, _load, _ptr
 
 __all__ = ["EmbeddingPlan", "embedding_lookup", "embedding_bag",
-           "embedding_plan", "embedding_grad"]
+           "embedding_plan", "embedding_grad", "MAX_TOKENS"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MAX_ROWS = 2 ** 31 - 2 ** 16     # of a table that is looked up
-_MAX = 2 ** 29                    # ids, bags and rows of a sum or gradient
+MAX_TOKENS = 2 ** 29              # ids, bags and rows of a sum or gradient
 _MAX_DIM = 2 ** 22
 
 
@@ -151,9 +151,9 @@ def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
                          f"length], got shape {tuple(ids.shape)}")
     kind, offsets, fixed, bags = _bags(ids, offsets, "embedding_bag")
     n = ids.numel()
-    if n > _MAX or bags > _MAX:
+    if n > MAX_TOKENS or bags > MAX_TOKENS:
         raise ValueError(f"embedding_bag: {n} ids in {bags} bags are over "
-                         f"{_MAX}")
+                         f"{MAX_TOKENS}")
     weights = _weights(weights, n, "embedding_bag.weights", table.device)
     V, D = table.shape
     if n == 0:
@@ -224,9 +224,9 @@ def embedding_plan(ids: torch.Tensor, num_rows: int,
     kind, fixed, bags = 0, 1, n
     if bagged:
         kind, offsets, fixed, bags = _bags(ids, offsets, "embedding_plan")
-    if not 0 <= V <= _MAX or n > _MAX or bags > _MAX:
+    if not 0 <= V <= MAX_TOKENS or n > MAX_TOKENS or bags > MAX_TOKENS:
         raise ValueError(f"embedding_plan: {n} ids in {bags} bags over {V} "
-                         f"rows are over {_MAX}")
+                         f"rows are over {MAX_TOKENS}")
     kept = torch.empty((3 if bagged else 2) * n + V + 1, dtype=torch.int32,
                        device=ids.device)
     need = lib.ks_token_sort_work(n, V)

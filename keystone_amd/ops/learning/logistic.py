@@ -14,7 +14,7 @@ from ...parallel.dataset import TensorDataset
 from ...workflow.pipeline import BatchTransformer, LabelEstimator
 from .lbfgs import DenseLBFGSwithL2, LogisticGradient, SparseLBFGSwithL2
 from .linear import LinearMapper
-from .sparse_rows import SparseRows
+from .sparse_rows import SparseRows, csr_matmul
 
 __all__ = ["LogisticRegressionEstimator", "LogisticRegressionModel",
            "NaiveBayesEstimator", "NaiveBayesModel"]
@@ -33,9 +33,7 @@ class LogisticRegressionModel(BatchTransformer):
     def apply_batch(self, X: torch.Tensor) -> torch.Tensor:
         self.W = self.W.to(device=X.device, dtype=X.dtype if X.dtype.is_floating_point else self.W.dtype)
         if SparseRows.supports(X):
-            from ... import hip
-            S = hip.embedding_bag(self.W, X.col_indices(), X.crow_indices(),
-                                  X.values())
+            S = csr_matmul(X, self.W)
         else:
             S = X @ self.W
         if self.b is not None:
@@ -87,10 +85,7 @@ class NaiveBayesModel(BatchTransformer):
         self.log_prior = self.log_prior.to(device=X.device)
         lt, lp = self.log_theta, self.log_prior
         if SparseRows.supports(X):
-            from ... import hip
-            return hip.embedding_bag(lt.to(X.dtype), X.col_indices(),
-                                     X.crow_indices(), X.values()
-                                     ) + lp.to(X.dtype)
+            return csr_matmul(X, lt.to(X.dtype)) + lp.to(X.dtype)
         if X.layout == torch.sparse_csr or X.is_sparse:
             return torch.sparse.mm(X, lt.to(X.dtype)) + lp.to(X.dtype)
         return X @ lt.to(X.dtype) + lp.to(X.dtype)

@@ -10,7 +10,19 @@ from __future__ import annotations
 
 import torch
 
-__all__ = ["SparseRows"]
+__all__ = ["SparseRows", "csr_matmul"]
+
+
+def csr_matmul(X: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
+    """``X @ W`` of CSR rows that ``SparseRows.supports``."""
+    # the kernels keep nothing for autograd, and take no shape that does not fit
+    if W.dim() != 2 or (W.requires_grad and torch.is_grad_enabled()):
+        return X @ W
+    if X.shape[1] != W.shape[0]:
+        raise RuntimeError(f"rows of {X.shape[1]} features by weights "
+                           f"{tuple(W.shape)}")
+    from ... import hip
+    return hip.embedding_bag(W, X.col_indices(), X.crow_indices(), X.values())
 
 
 class SparseRows:
@@ -30,11 +42,15 @@ class SparseRows:
 
     @staticmethod
     def supports(X: torch.Tensor) -> bool:
+        """Whether X is such rows, with sizes that the kernels take."""
         if not (X.layout == torch.sparse_csr and X.is_cuda
-                and X.dtype == torch.float32):
+                and X.dtype == torch.float32 and X.dim() == 2):
+            return False
+        if X.requires_grad and torch.is_grad_enabled():
             return False
         from ... import hip
-        return hip.gpu_ready()
+        return max(*X.shape, X.values().numel()) <= hip.MAX_TOKENS \
+            and hip.gpu_ready()
 
     def __matmul__(self, W: torch.Tensor) -> torch.Tensor:
         S = self.hip.embedding_bag(W[:self.features], self.columns,

@@ -14,6 +14,7 @@ from keystone_amd.ops.learning import (
     EmbeddingClassifierEstimator, LeastSquaresGradient, LinearMapEstimator,
     LinearMapper, LogisticGradient, MiniBatchSGDwithL2, QuantizedEstimator,
     QuantizedLinearMapper)
+from keystone_amd.ops.learning.sparse_rows import SparseRows
 from keystone_amd.ops.nlp import MeanEmbedding, PadTokens, TokenEmbedding
 from keystone_amd.ops.nlp.embedding import (embed_tokens, mean_weights,
                                             sum_tokens, token_table_grad)
@@ -312,3 +313,24 @@ def test_kernels_refuse_host_tensors():
                  lambda: hip.fp8_linear(T, hip.fp8_pack(torch.ones(3, 2)))):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_sparse_rows_over_the_kernels_sizes_are_left_to_torch(monkeypatch):
+    from types import SimpleNamespace
+    monkeypatch.setattr(hip, "gpu_ready", lambda: True)
+
+    def rows(n, d, entries, dims=2, grad=False):
+        return SimpleNamespace(
+            layout=torch.sparse_csr, is_cuda=True, dtype=torch.float32,
+            shape=(n, d), dim=lambda: dims, requires_grad=grad,
+            values=lambda: SimpleNamespace(numel=lambda: entries))
+
+    most = hip.MAX_TOKENS
+    assert SparseRows.supports(rows(most, most, most))
+    assert not SparseRows.supports(rows(most + 1, 5, 5))
+    assert not SparseRows.supports(rows(5, most + 1, 5))
+    assert not SparseRows.supports(rows(5, 5, most + 1))
+    assert not SparseRows.supports(rows(5, 5, 5, dims=3))
+    assert not SparseRows.supports(rows(5, 5, 5, grad=True))
+    with torch.no_grad():
+        assert SparseRows.supports(rows(5, 5, 5, grad=True))

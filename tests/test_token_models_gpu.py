@@ -10,7 +10,7 @@ from keystone_amd.ops.learning import (
     DenseLBFGSwithL2, EmbeddingClassifierEstimator, LeastSquaresGradient,
     LinearMapper, LogisticGradient, LogisticRegressionEstimator,
     LogisticRegressionModel, NaiveBayesModel, SparseLBFGSwithL2)
-from keystone_amd.ops.learning.sparse_rows import SparseRows
+from keystone_amd.ops.learning.sparse_rows import SparseRows, csr_matmul
 
 pytestmark = pytest.mark.gpu
 
@@ -42,6 +42,25 @@ def test_sparse_rows_multiply():
                 # at most 703 roundings in a sum
                 assert ((got.cpu().double() - want).abs()
                         <= 703 * 2.0 ** -24 * mag + 1e-30).all()
+
+
+def test_sparse_scores_keep_refusals_and_gradients():
+    X = sparse(30, 40, 0.2).to_sparse_csr().cuda()
+    for k in (39, 41):
+        with pytest.raises(RuntimeError):
+            csr_matmul(X, torch.randn(k, 3, device="cuda"))
+        with pytest.raises(RuntimeError):
+            LogisticRegressionModel(torch.randn(k, 3, device="cuda")
+                                    ).apply_batch(X)
+        with pytest.raises(RuntimeError):
+            NaiveBayesModel(torch.zeros(3, device="cuda"),
+                            torch.randn(k, 3, device="cuda")).apply_batch(X)
+    W = torch.randn(40, 3, device="cuda", requires_grad=True)
+    csr_matmul(X, W).sum().backward()
+    want = X.to_dense().cpu().double().sum(0)
+    assert torch.allclose(W.grad[:, 0].cpu().double(), want, atol=1e-5)
+    w = torch.randn(40, device="cuda")
+    assert csr_matmul(X, w).shape == (30,)
 
 
 @pytest.mark.parametrize("grad", [LeastSquaresGradient(), LogisticGradient()])
