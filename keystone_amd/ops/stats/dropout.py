@@ -40,7 +40,9 @@ def dropout(x: torch.Tensor, p: float, seed: int, step: int = 0
     """Zeros each element with chance ``p`` (to a multiple of 2^-16) and
     scales the others so that the mean stays."""
     from ... import hip
-    if x.is_cuda and x.dtype in (torch.float32, torch.bfloat16,
+    # the kernel keeps nothing for autograd
+    differentiated = x.requires_grad and torch.is_grad_enabled()
+    if not differentiated and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16,
                                  torch.float16) and hip.gpu_ready():
         return hip.dropout(x, p, seed, step)
     if not (0 <= seed < 2 ** 64 and 0 <= step < 2 ** 64):

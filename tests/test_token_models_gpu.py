@@ -11,6 +11,9 @@ from keystone_amd.ops.learning import (
     LinearMapper, LogisticGradient, LogisticRegressionEstimator,
     LogisticRegressionModel, NaiveBayesModel, SparseLBFGSwithL2)
 from keystone_amd.ops.learning.sparse_rows import SparseRows, csr_matmul
+from keystone_amd.ops.nlp.embedding import (embed_tokens, sum_tokens,
+                                            token_table_grad)
+from keystone_amd.ops.stats import dropout
 
 pytestmark = pytest.mark.gpu
 
@@ -270,3 +273,25 @@ def test_refusals():
             call()
             print("not refused:", k)
     torch.cuda.synchronize()
+
+
+def test_autograd_through_the_operators_is_not_lost():
+    """Sums of up to ten terms of at most 20: ten roundings of 2^-24 a side."""
+    g = torch.Generator().manual_seed(4)
+    table = torch.randn(20, 8, generator=g).cuda()
+    ids = torch.randint(-1, 21, (6, 5), generator=g).cuda()
+    w = torch.rand(6, 5, generator=g).cuda()
+    dy = torch.randn(6, 8, generator=g).cuda()
+    t, v = table.clone().requires_grad_(), w.clone().requires_grad_()
+    y = dropout(sum_tokens(t, ids, v, 0.5), 0.3, 11, 2)
+    y.backward(dy)
+    assert torch.allclose(y, dropout(sum_tokens(table, ids, w, 0.5), 0.3, 11, 2),
+                          atol=4e-5)
+    dh = dropout(dy, 0.3, 11, 2)
+    assert torch.allclose(t.grad, token_table_grad(dh, ids, 20, w, 0.5),
+                          atol=4e-5)
+    want = 0.5 * (embed_tokens(table, ids) * dh.unsqueeze(1)).sum(-1)
+    assert torch.allclose(v.grad, want, atol=4e-5)
+    with torch.no_grad():
+        assert torch.equal(sum_tokens(t, ids, v, 0.5),
+                           hip.embedding_bag(table, ids, None, w, 0.5))
