@@ -28,7 +28,8 @@ def dropout(x: torch.Tensor, p: float, seed: int,
     """Zeros each element with chance ``p`` and scales the others so that the
     mean stays.  Which ones is a function of ``(seed, step)`` and the
     element's place in ``x`` alone: the gradient is ``dropout(dy, p, seed,
-    step)``, and no mask is kept.  What is dropped is zero whatever it held.
+    step)``, and no mask is kept, nor anything for autograd.  What is dropped is
+    zero whatever it held.
 
     ``step``: a number below 2^64, or an int64 tensor of one element on x's
     device, which a captured graph reads at each replay.  ``out`` may be

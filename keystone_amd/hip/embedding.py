@@ -11,7 +11,7 @@ and weights) the bag sum is ``X @ T`` and the gradient ``X.T @ dY``.
 
 Tables and gradients are float32, bfloat16 or float16 with unit inner stride;
 sums are held in float32 and rounded once.  Every sum has one order, so two
-runs give the same bits.
+runs give the same bits.  Nothing is kept for autograd: the gradient is a call.
 """
 
 from __future__ import annotations

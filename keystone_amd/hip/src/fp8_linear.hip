@@ -745,7 +745,7 @@ int rows_per(int M, int N, int kblocks) {
     return per_split(kblocks, rows_splits(M, N, kblocks));
 }
 
-constexpr int MOST_NARROW = 10;
+constexpr int MOST_NARROW = 10, MOST_ROWS = 1 << 25;
 
 // Tiles of rows in a block of fp8_narrow_kernel: two read W half as often, where
 // that leaves work for each compute unit.  bf16, one tile and two: 8192 x 8192 x
@@ -763,7 +763,8 @@ enum Kind { STAGED, NARROW, ROWS, TILES, LARGE };
 
 Kind kind_of(int type, int M, int N, int kblocks) {
     const int mt = ks_ceil_div(M, 16), nt = ks_ceil_div(N, 16);
-    const bool few = mt == 1 || (long long)mt * nt <= 512 || (mt <= 64 && nt <= 16);
+    const bool few = (mt == 1 && nt < (1 << 21)) || (long long)mt * nt <= 512 ||
+                     (mt <= 64 && nt <= 16);
     // 1 x 16384 x 1000 f32: 7.9 us staged, 10.9 us with a launch for X; 128 x
     // 2048 x 1000 7.9 and 7.5 us, but 9.2 and 12 us with the host's part.  1021 x
     // 2048 x 147 7.4 us, 10.6 us by NARROW; 2048 rows 17.5 and 11 us.
@@ -844,8 +845,15 @@ void narrow(const Gemm& a, const Rows<T>& src, T* y, float* part,
                            : fp8_narrow_kernel<T, 1, 5>;
     if constexpr (sizeof(T) == 2)
         if (down == 2) kernel = fp8_narrow_kernel<T, 2, MOST_NARROW>;
-    kernel<<<dim3(ks_ceil_div(a.M, 16 * down), splits), 64 * narrow_waves(down), 0,
-             stream>>>(a, src, y, part, bias, kper);
+    // a launch has fewer than 2^32 threads
+    for (long long m = 0; m < a.M; m += MOST_ROWS) {
+        Gemm some = a;
+        some.M = (int)(a.M - m < MOST_ROWS ? a.M - m : MOST_ROWS);
+        kernel<<<dim3(ks_ceil_div(some.M, 16 * down), splits),
+                 64 * narrow_waves(down), 0, stream>>>(
+            some, Rows<T>{src.x + m * src.ld, src.ld, src.K}, y + m * a.N, part,
+            bias, kper);
+    }
 }
 
 template <typename T>

@@ -157,6 +157,63 @@ def test_strided_and_misaligned_rows(hip):
           base[:, :300], W[:, ::2], None)
 
 
+@pytest.mark.parametrize("M,pitch,K", [(600, 2 ** 22, 900), (1100, 2 ** 21, 900),
+                                       (600, 2 ** 22, 5000)])
+def test_rows_past_32_bit_offsets(hip, M, pitch, K):
+    """Staged, narrow and quantised apart, each from 4.6 GB and more of rows."""
+    W = torch.randn(K, 40, device="cuda")
+    packed = hip.fp8_pack(W)
+    base = torch.zeros(M, pitch, dtype=torch.bfloat16, device="cuda")
+    X = base[:, pitch - K:]
+    X.copy_(torch.randn(M, K, device="cuda"))
+    got = hip.fp8_linear(X, packed)
+    assert torch.equal(got, hip.fp8_linear(X.contiguous(), packed))
+    check(hip, got[-20:], X[-20:].contiguous(), W, None)
+
+
+def test_more_rows_than_a_launch_takes(hip):
+    M, K, N = 2 ** 25 + 37, 3, 2
+    X = torch.randn(M, K, device="cuda").to(torch.bfloat16)
+    W = torch.randn(K, N, device="cuda")
+    got = hip.fp8_linear(X, hip.fp8_pack(W))
+    for a, b in ((0, 100), (2 ** 25 - 50, 2 ** 25 + 37), (2 ** 24, 2 ** 24 + 100)):
+        check(hip, got[a:b], X[a:b], W, None)
+
+
+def test_wide_weights_of_few_rows(hip):
+    N = 2 ** 25 + 21
+    W = torch.randn(2, N, device="cuda").to(torch.bfloat16)
+    X = torch.randn(3, 2, device="cuda").to(torch.bfloat16)
+    got = hip.fp8_linear(X, hip.fp8_pack(W))
+    for a, b in ((0, 100), (N - 100, N)):
+        check(hip, got[:, a:b], X, W[:, a:b], None)
+
+
+def test_two_streams_at_once(hip):
+    """Calls in flight together, each on its own stream, share nothing."""
+    sets = [operands(M, K, N, torch.float32, seed) for seed, (M, K, N) in
+            enumerate([(1021, 8192, 147), (1100, 9000, 120), (16, 8192, 1000),
+                       (200, 4096, 130)])]
+    packed = [hip.fp8_pack(W) for _, W, _ in sets]
+    want = [hip.fp8_linear(X, P, b) for (X, _, b), P in zip(sets, packed)]
+    ids = [torch.randint(0, 5000, (n,), device="cuda") for n in
+           (777, 9000, 70001, 5000)]
+    plans = [hip.embedding_plan(i, 5000) for i in ids]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got, order = [], []
+        for st, (X, _, b), P, i in zip(streams, sets, packed, ids):
+            with torch.cuda.stream(st):
+                got.append(hip.fp8_linear(X, P, b))
+                order.append(hip.embedding_plan(i, 5000).order.clone())
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+        for a, p in zip(order, plans):
+            assert torch.equal(a, p.order)
+
+
 def test_empty(hip):
     W = hip.fp8_pack(torch.randn(40, 6, device="cuda"))
     assert hip.fp8_linear(torch.empty(0, 40, device="cuda"), W).shape == (0, 6)
