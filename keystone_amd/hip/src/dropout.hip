@@ -35,7 +35,7 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0,
 
 template <typename T>
 __global__ __launch_bounds__(256)
-void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long long n,
+void dropout_kernel(const T* x, T* y, long long n,   // y may be x
                     uint32_t threshold, float scale, uint64_t seed,
                     uint64_t step, const long long* __restrict__ step_at,
                     long long first) {
