@@ -111,13 +111,14 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     if n and D:
         _launch("ks_embedding_lookup", table.device, ids.data_ptr(),
                 ids.dtype == torch.int64, n, table.data_ptr(),
-                _TYPES[table.dtype], V, _pitch(table), out.data_ptr(), D,
-                scale, _width(D, table.element_size()))
+                _TYPES[table.dtype], V, table.stride(0) if V > 1 else D,
+                out.data_ptr(), D, scale, _width(D, table.element_size()))
     return out
 
 
 def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
                  weights, keys, src, out, scale, accumulate):
+    """V: src's rows, count: out's."""
     D = out.shape[1]
     if count == 0 or D == 0:
         return
@@ -125,11 +126,12 @@ def _segment_sum(lib, kind, bounds, fixed, count, n, ids, ids_wide, V, order,
     work = None
     need = lib.ks_segment_work(n, D, vec, keys is not None)
     if need:
-        work = torch.empty(need, dtype=torch.float32, device=src.device)
+        work = src.new_empty(need, dtype=torch.float32)
     _launch("ks_segment_sum", src.device, kind, bounds, fixed, count, n, ids,
             ids_wide, V, order, _ptr(weights), keys, src.data_ptr(),
-            _TYPES[src.dtype], _pitch(src), out.data_ptr(), _TYPES[out.dtype],
-            _pitch(out), _ptr(work), D, scale, accumulate, vec)
+            _TYPES[src.dtype], src.stride(0) if V > 1 else D, out.data_ptr(),
+            _TYPES[out.dtype], out.stride(0) if count > 1 else D, _ptr(work), D,
+            scale, accumulate, vec)
 
 
 def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
@@ -158,7 +160,7 @@ def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
     V, D = table.shape
     if n == 0:
         return torch.zeros(bags, D, dtype=table.dtype, device=table.device)
-    out = torch.empty(bags, D, dtype=table.dtype, device=table.device)
+    out = table.new_empty((bags, D))
     _segment_sum(lib, kind, _ptr(offsets), fixed, bags, n, ids.data_ptr(),
                  ids.dtype == torch.int64, V, None, weights, None, table, out,
                  scale, False)
@@ -227,11 +229,9 @@ def embedding_plan(ids: torch.Tensor, num_rows: int,
     if not 0 <= V <= MAX_TOKENS or n > MAX_TOKENS or bags > MAX_TOKENS:
         raise ValueError(f"embedding_plan: {n} ids in {bags} bags over {V} "
                          f"rows are over {MAX_TOKENS}")
-    kept = torch.empty((3 if bagged else 2) * n + V + 1, dtype=torch.int32,
-                       device=ids.device)
+    kept = ids.new_empty((3 if bagged else 2) * n + V + 1, dtype=torch.int32)
     need = lib.ks_token_sort_work(n, V)
-    work = torch.empty(need, dtype=torch.int32, device=ids.device) \
-        if need else None
+    work = ids.new_empty(need, dtype=torch.int32) if need else None
     plan = EmbeddingPlan(kept, V, bags, n, bagged)
     keys, order, rows, starts = plan._places()
     _launch("ks_token_sort", ids.device, ids.data_ptr(),
@@ -272,7 +272,7 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
         if dtype not in _TYPES:
             raise RuntimeError(f"embedding_grad: expected float32, bfloat16 "
                                f"or float16, got {dtype}")
-        out = torch.empty(shape, dtype=dtype, device=grad.device)
+        out = grad.new_empty(shape, dtype=dtype)
     else:
         if out.shape != shape:
             raise ValueError(f"embedding_grad.out: expected shape {shape}, "
