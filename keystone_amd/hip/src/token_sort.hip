@@ -11,8 +11,8 @@
 // each one's place is counted instead, in one launch.
 //
 // Bound by latency and launches, tokens of 100000: 777 take 4.7 us, 4096 take
-// 8.2 us, 16384 take 29 us in seven launches, 1048576 take 56 us (78 us with
-// scattered writes of 4 bytes), 8388608 take 198 us.
+// 8.2 us, 16384 take 27 us in seven launches, 1048576 take 52 us (78 us with
+// scattered writes of 4 bytes), 8388608 take 175 us.
 #include "common.h"
 
 #include <cstdint>
@@ -21,10 +21,10 @@ namespace {
 
 constexpr int WAVES = 4;
 // A tile's tokens are so many for each of its block's threads.  Few of them
-// fill the card with few tokens: 65536 take 32 us with two a thread, 53 us
-// with eight, 262144 take 38 and 42 us, 400000 take 49 and 44 us.
+// fill the card with few tokens: 65536 take 30 us with two a thread, 50 us
+// with eight, 262144 take 32 and 39 us, 524288 take 42 and 41 us.
 constexpr int FEW = 2, MANY = 8;
-constexpr int ROUNDS_LIMIT = 262144;
+constexpr int ROUNDS_LIMIT = 524288;
 
 int rounds_of(int n) { return n <= ROUNDS_LIMIT ? FEW : MANY; }
 
@@ -79,8 +79,8 @@ __device__ __forceinline__ int max_block(int x, int* wave_max) {
 
 // The bags of a tile's positions, -1 outside: every bag that begins in the tile
 // marks its first position, and a position's bag is the last mark so far.
-// 524288 tokens in bags of ten are sorted in 59 us, in 69 us where each
-// position searches the bounds.
+// 524288 tokens in bags of ten were sorted in 59 us with them, in 69 us where
+// each position searched the bounds; now 53 us.
 template <int ROUNDS>
 __device__ __forceinline__ void bags_of_tile(const Bags& bags, int n,
                                              long long first,
@@ -141,7 +141,7 @@ __device__ __forceinline__ void bags_of_tile(const Bags& bags, int n,
 template <int ROUNDS>
 __global__ __launch_bounds__(256)
 void digit_count_kernel(Source src, int shift, int bits,
-                        int* __restrict__ counts, int tiles, Bags bags) {
+                        int* __restrict__ counts, Bags bags) {
     __shared__ int bin[MAX_BINS];
     const int bins = 1 << bits;
     const long long first = (long long)blockIdx.x * (ROUNDS * 256);
@@ -162,38 +162,48 @@ void digit_count_kernel(Source src, int shift, int bits,
         if (first + r * 256 + threadIdx.x < src.n) atomicAdd(&bin[digit[r]], 1);
     __syncthreads();
     for (int i = threadIdx.x; i < bins; i += 256)
-        counts[(long long)i * tiles + blockIdx.x] = bin[i];
+        counts[(long long)blockIdx.x * bins + i] = bin[i];
 }
 
-// Exclusive sums over the tiles of one digit, in place, and its total.
-__global__ __launch_bounds__(256)
-void digit_scan_kernel(int* __restrict__ counts, int tiles,
+// Exclusive sums over the tiles, in place, and each digit's total.  counts are
+// [tile][digit], so that a tile writes and reads its own in whole lines (8388608
+// tokens take 175 us, 200 us with [digit][tile]); a block has 16 digits, and 64
+// groups of lanes a stretch of the tiles each.
+__global__ __launch_bounds__(1024)
+void digit_scan_kernel(int* __restrict__ counts, int tiles, int bins,
                        int* __restrict__ totals) {
-    __shared__ int wave_sum[4];
-    int* row = counts + (long long)blockIdx.x * tiles;
+    __shared__ int part[64][17];
+    const int digit = blockIdx.x * 16 + (threadIdx.x & 15), group = threadIdx.x >> 4;
+    const int each = (tiles + 63) / 64;
+    const int t0 = min(tiles, group * each), t1 = min(tiles, t0 + each);
+    int* const at = counts + digit;
+    int sum = 0;
+    if (digit < bins)
+#pragma unroll 4
+        for (int t = t0; t < t1; ++t) sum += at[(long long)t * bins];
+    part[group][threadIdx.x & 15] = sum;
+    __syncthreads();
+    // a wave scans one digit's 64 groups
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int carry = 0;
-    for (int first = 0; first < tiles; first += 256) {
-        const int i = first + threadIdx.x;
-        const int x = i < tiles ? row[i] : 0;
-        int s = x;
+    const int x = part[lane][wave];
+    int s = x;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(s, d, 64);
-            if (lane >= d) s += y;
-        }
-        if (lane == 63) wave_sum[wave] = s;
-        __syncthreads();
-        int before = carry, all = 0;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) before += wave_sum[w];
-            all += wave_sum[w];
-        }
-        if (i < tiles) row[i] = before + s - x;
-        carry += all;
-        __syncthreads();
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(s, d, 64);
+        if (lane >= d) s += y;
     }
-    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+    part[lane][wave] = s - x;
+    if (lane == 63 && blockIdx.x * 16 + wave < bins)
+        totals[blockIdx.x * 16 + wave] = s;
+    __syncthreads();
+    int before = part[group][threadIdx.x & 15];
+    if (digit < bins)
+#pragma unroll 4
+        for (int t = t0; t < t1; ++t) {
+            const int c = at[(long long)t * bins];
+            at[(long long)t * bins] = before;
+            before += c;
+        }
 }
 
 // The lanes of this wave whose digit equals this lane's.
@@ -246,7 +256,7 @@ __device__ __forceinline__ int scan_block(int x, int* wave_sum) {
 template <int ROUNDS>
 __global__ __launch_bounds__(256)
 void digit_move_kernel(Source src, int shift, int bits,
-                       const int* __restrict__ counts, int tiles,
+                       const int* __restrict__ counts,
                        const int* __restrict__ totals,
                        int2* __restrict__ pairs_out, int* __restrict__ keys,
                        int* __restrict__ order, int* __restrict__ rows) {
@@ -271,8 +281,9 @@ void digit_move_kernel(Source src, int shift, int bits,
     // two digits a thread
     const int d0 = threadIdx.x * 2, d1 = d0 + 1;
     const int t0 = d0 < bins ? totals[d0] : 0, t1 = d1 < bins ? totals[d1] : 0;
-    const int c0 = d0 < bins ? counts[(long long)d0 * tiles + blockIdx.x] : 0;
-    const int c1 = d1 < bins ? counts[(long long)d1 * tiles + blockIdx.x] : 0;
+    const int* const mine_at = counts + (long long)blockIdx.x * bins;
+    const int c0 = d0 < bins ? mine_at[d0] : 0;
+    const int c1 = d1 < bins ? mine_at[d1] : 0;
     const int global = scan_block(t0 + t1, wave_sum);
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r)
@@ -328,7 +339,7 @@ void digit_move_kernel(Source src, int shift, int bits,
 // before it, counted against all of them in LDS by 16 lanes.  n^2 comparisons
 // are less than the passes' barriers: two instructions each, over the whole
 // card.  Further blocks count the tokens below each of STARTS ids.  8192
-// tokens take 15 us, 29 us by digits; 16384 take 77 and 29 us.
+// tokens take 15 us, 27 us by digits; 16384 take 77 and 27 us.
 constexpr int SMALL = 8192, PLACED = 16, STARTS = 2048;
 
 __global__ __launch_bounds__(256)
@@ -427,7 +438,7 @@ void small_sort_kernel(const void* __restrict__ ids, int wide, int n, int V,
 }
 
 // starts[v]: how many sorted keys are below v.  Three keys a step, loaded without
-// a branch so that they overlap: the plan of 131072 tokens takes 34.5 us, 35.7 us
+// a branch so that they overlap: the plan of 131072 tokens takes 1 us less than
 // with a binary search.
 __global__ __launch_bounds__(256)
 void token_starts_kernel(const int* __restrict__ keys, int n, int V,
@@ -471,10 +482,11 @@ void sort_by_digits(Source src, const Bags& bags, int* keys, int* order,
     for (int p = 0; p < passes; ++p) {
         int2* to = p == passes - 1 ? nullptr : pairs[p & 1];
         digit_count_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
-            src, p * bits, bits, counts, tiles, bags);
-        digit_scan_kernel<<<1 << bits, 256, 0, stream>>>(counts, tiles, totals);
+            src, p * bits, bits, counts, bags);
+        digit_scan_kernel<<<ks_ceil_div(1 << bits, 16), 1024, 0, stream>>>(
+            counts, tiles, 1 << bits, totals);
         digit_move_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
-            src, p * bits, bits, counts, tiles, totals, to, keys, order, rows);
+            src, p * bits, bits, counts, totals, to, keys, order, rows);
         src.pairs = to;
     }
 }

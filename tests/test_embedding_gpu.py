@@ -178,7 +178,7 @@ def test_plan_is_a_stable_sort(hip, n, V):
 
 @pytest.mark.parametrize("V", [1, 2047, 2048, 100001])
 @pytest.mark.parametrize("n", [17, 4000, 8191, 8192, 8193, 70001, 262144,
-                               262145, 400001])
+                               262145, 400001, 524288, 524289])
 @pytest.mark.parametrize("bags", ["most of them empty", "long", "one", "ten",
                                   "all empty", "fixed"])
 def test_plan_of_bags(hip, n, V, bags):
