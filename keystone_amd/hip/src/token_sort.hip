@@ -11,7 +11,7 @@
 // each one's place is counted instead, in one launch.
 //
 // Bound by latency and launches, tokens of 100000: 777 take 4.7 us, 4096 take
-// 8.2 us, 16384 take 27 us in seven launches, 1048576 take 52 us (78 us with
+// 8.2 us, 16384 take 25 us in five launches, 1048576 take 52 us (78 us with
 // scattered writes of 4 bytes), 8388608 take 175 us.
 #include "common.h"
 
@@ -25,6 +25,12 @@ constexpr int WAVES = 4;
 // with eight, 262144 take 32 and 39 us, 524288 take 42 and 41 us.
 constexpr int FEW = 2, MANY = 8;
 constexpr int ROUNDS_LIMIT = 524288;
+
+// Up to so many tiles each sums all tiles' counts itself, without the scan's
+// launch: 12000 tokens in bags take 24.2 us, 26.5 us with it, and a launch less on
+// the host; 32768 take 25.1 and 23.6 us, but 39 and 40 us with the host's part and
+// the gradient's; 65536, of 128 tiles, 36.7 and 29.5 us.
+constexpr int UNSCANNED = 64;
 
 int rounds_of(int n) { return n <= ROUNDS_LIMIT ? FEW : MANY; }
 
@@ -280,10 +286,25 @@ void digit_move_kernel(Source src, int shift, int bits,
         for (int w = 0; w < WAVES; ++w) count[w][i] = 0;
     // two digits a thread
     const int d0 = threadIdx.x * 2, d1 = d0 + 1;
-    const int t0 = d0 < bins ? totals[d0] : 0, t1 = d1 < bins ? totals[d1] : 0;
-    const int* const mine_at = counts + (long long)blockIdx.x * bins;
-    const int c0 = d0 < bins ? mine_at[d0] : 0;
-    const int c1 = d1 < bins ? mine_at[d1] : 0;
+    int t0 = 0, t1 = 0, c0 = 0, c1 = 0;
+    if (d0 < bins) {
+        const int2* const at = (const int2*)(counts + d0);
+        if (totals) {
+            const int2 t = *(const int2*)(totals + d0);
+            const int2 c = at[(long long)blockIdx.x * (bins / 2)];
+            t0 = t.x, t1 = t.y, c0 = c.x, c1 = c.y;
+        } else {
+            // not scanned: all tiles' counts are summed here
+#pragma unroll 8
+            for (int k = 0; k < (int)gridDim.x; ++k) {
+                const int2 c = at[k * (bins / 2)];
+                t0 += c.x;
+                t1 += c.y;
+                c0 += k < (int)blockIdx.x ? c.x : 0;
+                c1 += k < (int)blockIdx.x ? c.y : 0;
+            }
+        }
+    }
     const int global = scan_block(t0 + t1, wave_sum);
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r)
@@ -339,7 +360,7 @@ void digit_move_kernel(Source src, int shift, int bits,
 // before it, counted against all of them in LDS by 16 lanes.  n^2 comparisons
 // are less than the passes' barriers: two instructions each, over the whole
 // card.  Further blocks count the tokens below each of STARTS ids.  8192
-// tokens take 15 us, 27 us by digits; 16384 take 77 and 27 us.
+// tokens take 15 us, 20 us by digits; 16384 take 77 and 25 us.
 constexpr int SMALL = 8192, PLACED = 16, STARTS = 2048;
 
 __global__ __launch_bounds__(256)
@@ -483,10 +504,12 @@ void sort_by_digits(Source src, const Bags& bags, int* keys, int* order,
         int2* to = p == passes - 1 ? nullptr : pairs[p & 1];
         digit_count_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
             src, p * bits, bits, counts, bags);
-        digit_scan_kernel<<<ks_ceil_div(1 << bits, 16), 1024, 0, stream>>>(
-            counts, tiles, 1 << bits, totals);
+        if (tiles > UNSCANNED)
+            digit_scan_kernel<<<ks_ceil_div(1 << bits, 16), 1024, 0, stream>>>(
+                counts, tiles, 1 << bits, totals);
         digit_move_kernel<ROUNDS><<<tiles, 256, 0, stream>>>(
-            src, p * bits, bits, counts, totals, to, keys, order, rows);
+            src, p * bits, bits, counts, tiles > UNSCANNED ? totals : nullptr, to,
+            keys, order, rows);
         src.pairs = to;
     }
 }
