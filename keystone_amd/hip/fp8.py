@@ -27,7 +27,7 @@ _MAX_INNER = 2 ** 26
 class Fp8Weight:
     """``W`` [K, N] in 8 bits, laid out as the matrix instruction reads it:
     ``data`` [N/16, K/128, 2048] bytes and ``scales`` [N/16, K/512, 64]
-    bytes, 127 + exponent, with sides rounded up."""
+    bytes, 127 + exponent (127 past the end), with sides rounded up."""
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, K: int,
                  N: int):

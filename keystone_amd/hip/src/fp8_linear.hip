@@ -138,9 +138,14 @@ void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
     unsigned char* to = q + chunk * CHUNK + lane * 16;
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(to + 1024) = make_uint4(w[4], w[5], w[6], w[7]);
-    if (lane < 16)
-        scales[((long long)tile * ((kblocks + 3) / 4) + kb / 4) * 64 +
-               lane * 4 + (kb & 3)] = (unsigned char)e;
+    if (lane < 16) {
+        unsigned char* at = scales +
+            ((long long)tile * ((kblocks + 3) / 4) + kb / 4) * 64 + lane * 4;
+        at[kb & 3] = (unsigned char)e;
+        // a word's bytes past K are no block's, and saved along with the others
+        if (kb == kblocks - 1)
+            for (int b = (kb & 3) + 1; b < 4; ++b) at[b] = 127;
+    }
 }
 
 struct Gemm {

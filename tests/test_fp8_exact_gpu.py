@@ -153,3 +153,18 @@ def test_what_the_matrix_unit_cuts(hip, dtype, M):
                 kept = 126 if a <= 13 else 126 - alone
                 want = torch.tensor(sign * kept * 2.0 ** -a).to(dtype)
                 assert got.cpu().eq(want).all(), (one, other, a, sign)
+
+
+@pytest.mark.parametrize("K", [1, 128, 129, 300, 511, 513, 640, 1100])
+def test_packed_scales_are_whole(hip, K):
+    """Bytes of blocks past K's end are written too, so that two saves of one
+    matrix are the same and hold nothing of what memory held before."""
+    W = torch.randn(K, 33, generator=torch.Generator().manual_seed(K))
+    host = hip.fp8_pack(W)
+    # what is freed here is what the next tensors of these sizes get
+    for t in [torch.full_like(t, 0xab, device="cuda") for t in
+              (host.data, host.scales)]:
+        del t
+    packed = hip.fp8_pack(W.cuda())
+    assert torch.equal(packed.scales.cpu(), host.scales)
+    assert torch.equal(packed.data.cpu(), host.data)
