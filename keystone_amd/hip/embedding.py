@@ -16,6 +16,7 @@ runs give the same bits.  Nothing is kept for autograd: the gradient is a call.
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -255,8 +256,8 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
     step of gradient descent is ``embedding_grad(dY, plan, scale=-rate,
     out=table, accumulate=True)``."""
     lib = _load()
-    if grad.dim() > 2:
-        grad = grad.reshape(-1, grad.shape[-1])
+    if grad.dim() != 2 and grad.dim():     # rows may have no columns
+        grad = grad.reshape(math.prod(grad.shape[:-1]), grad.shape[-1])
     grad = _matrix(grad, "embedding_grad.grad")
     if grad.device != plan.device:
         raise RuntimeError(f"embedding_grad.grad: expected a tensor on "

@@ -1,0 +1,42 @@
+"""The token, dropout and 8-bit operators on the GPU at their edges: shapes,
+types and transforms that the CPU path takes and the kernels' path has to take
+alike, and sizes that reach the kernels' large and in-place variants."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from keystone_amd.ops.learning import LinearMapper
+from keystone_amd.ops.learning.sparse_rows import csr_matmul
+from keystone_amd.ops.nlp.embedding import (embed_tokens, sum_tokens,
+                                            token_table_grad)
+from keystone_amd.ops.stats import dropout
+from tests.test_embedding_gpu import check, gen, some_ids, some_offsets, sums64
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from keystone_amd import hip as h
+    assert h.available(), "HIP extension must be built and loadable"
+    return h
+
+
+# ------------------------------------------------------------ types, shapes
+def test_gradient_of_a_single_lookup(hip):
+    """Ids of no dimension, and rows of no columns."""
+    T = torch.randn(5, 3, device="cuda")
+    one = torch.tensor(2, device="cuda")
+    y = hip.embedding_lookup(T, one)
+    assert torch.equal(y, T[2])
+    d = hip.embedding_grad(y, hip.embedding_plan(one, 5))
+    want = torch.zeros(5, 3, device="cuda")
+    want[2] = T[2]
+    assert torch.equal(d, want)
+    ids = torch.zeros(2, 4, dtype=torch.int64, device="cuda")
+    y = hip.embedding_lookup(T[:, :0], ids)
+    assert y.shape == (2, 4, 0)
+    assert hip.embedding_grad(y, hip.embedding_plan(ids, 5)).shape == (5, 0)
