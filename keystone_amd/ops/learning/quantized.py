@@ -48,11 +48,12 @@ class QuantizedLinearMapper(BatchTransformer):
         if X.is_cuda and hip.gpu_ready():
             if X.dtype in (torch.float32, torch.bfloat16, torch.float16):
                 return hip.fp8_linear(X, self.packed, self.b)
-            return hip.fp8_linear(X.to(torch.float32), self.packed,
-                                  self.b).to(X.dtype)
-        out = hip.fp8_round(X) @ self.packed.dequantise()
-        if self.b is not None:
-            out = out + self.b
+            out = hip.fp8_linear(X.to(torch.float32), self.packed, self.b)
+        else:
+            out = hip.fp8_round(X) @ self.packed.dequantise()
+            if self.b is not None:
+                out = out + self.b
+        # whole numbers' scores are none
         return out.to(X.dtype) if X.is_floating_point() else out
 
     def apply(self, x):

@@ -25,6 +25,22 @@ def hip():
     return h
 
 
+# ------------------------------------------------------------- 8-bit mapper
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.uint8])
+def test_quantized_scores_of_whole_number_features(dtype):
+    """Counts as features: the scores are numbers with fractions, as on the
+    CPU, and not cut to whole ones."""
+    g = gen(1)
+    X = torch.randint(0, 9, (20, 200), generator=g).to(dtype)
+    q = LinearMapper(torch.randn(200, 7, generator=g),
+                     torch.randn(7, generator=g)).quantize()
+    want = q.apply_batch(X)
+    got = q.apply_batch(X.cuda())
+    assert got.dtype == want.dtype == torch.float32
+    # 202 roundings of sums of 200 products of at most 8 by 4
+    assert torch.allclose(got.cpu(), want, rtol=0, atol=202 * 2 ** -24 * 6400)
+
+
 # ------------------------------------------------------------ types, shapes
 def test_gradient_of_a_single_lookup(hip):
     """Ids of no dimension, and rows of no columns."""
