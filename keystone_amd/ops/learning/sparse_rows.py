@@ -10,13 +10,15 @@ from __future__ import annotations
 
 import torch
 
+from ...utils.derivatives import differentiated
+
 __all__ = ["SparseRows", "csr_matmul"]
 
 
 def csr_matmul(X: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
     """``X @ W`` of CSR rows that ``SparseRows.supports``."""
     # the kernels keep nothing for autograd, and take no shape that does not fit
-    if W.dim() != 2 or (W.requires_grad and torch.is_grad_enabled()):
+    if W.dim() != 2 or differentiated(W):
         return X @ W
     if X.shape[1] != W.shape[0]:
         raise RuntimeError(f"rows of {X.shape[1]} features by weights "

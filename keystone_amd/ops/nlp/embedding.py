@@ -5,7 +5,7 @@ nodes.nlp.WordFrequencyEncoder), -1 for an unseen word.  An id outside the
 table stands for no word: zeros from a lookup, no term of a mean, no
 gradient.  On the GPU these run as the kernels of ``keystone_amd.hip``, which
 keep nothing for autograd: solvers call ``token_table_grad``.  Where a table or
-weights ask for their gradient it is plain torch, as on the CPU.
+weights are differentiated it is plain torch, as on the CPU.
 """
 
 from __future__ import annotations
@@ -15,16 +15,16 @@ from typing import Optional, Sequence
 import torch
 
 from ...parallel.dataset import Dataset, TensorDataset
+from ...utils.derivatives import differentiated
 from ...workflow.pipeline import BatchTransformer, Transformer
 
 __all__ = ["PadTokens", "TokenEmbedding", "MeanEmbedding", "embed_tokens",
            "sum_tokens", "token_table_grad", "mean_weights"]
 
 
-def _hip(t: torch.Tensor, weights: Optional[torch.Tensor] = None):
+def _hip(t: torch.Tensor, *others: Optional[torch.Tensor]):
     """The kernels, where t's device and type go through them."""
-    if torch.is_grad_enabled() and (t.requires_grad or (
-            weights is not None and weights.requires_grad)):
+    if differentiated(t, *others):
         return None
     if t.is_cuda and t.dtype in (torch.float32, torch.bfloat16,
                                  torch.float16):
@@ -41,7 +41,7 @@ def _seen(ids: torch.Tensor, rows: int) -> torch.Tensor:
 def embed_tokens(table: torch.Tensor, ids: torch.Tensor,
                  scale: float = 1.0) -> torch.Tensor:
     """``scale * table[ids]``, [*ids.shape, D]."""
-    hip = _hip(table)
+    hip = _hip(table, ids)
     if hip is not None:
         return hip.embedding_lookup(table, ids, scale)
     seen = _seen(ids, table.shape[0])
@@ -55,7 +55,7 @@ def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
                scale: float = 1.0) -> torch.Tensor:
     """``scale * sum_j weights[b, j] table[ids[b, j]]``, [B, D], of ids
     [B, L]."""
-    hip = _hip(table, weights)
+    hip = _hip(table, ids, weights)
     if hip is not None:
         return hip.embedding_bag(table, ids, None, weights, scale)
     rows = embed_tokens(table, ids)
@@ -70,7 +70,7 @@ def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
                      ) -> torch.Tensor:
     """``sum_tokens``'s gradient with respect to the table, [num_rows, D];
     with ``out`` it is added to ``out``."""
-    hip = _hip(grad, weights)
+    hip = _hip(grad, ids, weights)
     if hip is not None:
         plan = hip.embedding_plan(ids, num_rows, pooled=True)
         return hip.embedding_grad(grad, plan, weights, scale, out=out,

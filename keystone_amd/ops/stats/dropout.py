@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import torch
 
+from ...utils.derivatives import differentiated
+
 __all__ = ["dropout"]
 
 _LOW = 0xFFFFFFFF
@@ -41,9 +43,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, step: int = 0
     scales the others so that the mean stays."""
     from ... import hip
     # the kernel keeps nothing for autograd
-    differentiated = x.requires_grad and torch.is_grad_enabled()
-    if not differentiated and x.is_cuda and x.dtype in (torch.float32, torch.bfloat16,
-                                 torch.float16) and hip.gpu_ready():
+    if x.is_cuda and x.dtype in (torch.float32, torch.bfloat16, torch.float16) \
+            and not differentiated(x) and hip.gpu_ready():
         return hip.dropout(x, p, seed, step)
     if not (0 <= seed < 2 ** 64 and 0 <= step < 2 ** 64):
         raise ValueError("dropout: expected a seed and a step in [0, 2^64), "

@@ -41,6 +41,57 @@ def test_quantized_scores_of_whole_number_features(dtype):
     assert torch.allclose(got.cpu(), want, rtol=0, atol=202 * 2 ** -24 * 6400)
 
 
+# --------------------------------------------------------------- transforms
+def test_tangents_go_through():
+    """Forward mode: a dual tensor asks for no gradient in reverse, and its
+    tangent is as on the CPU."""
+    g = gen(3)
+    T, dT = torch.randn(2, 20, 8, generator=g)
+    ids = torch.randint(-1, 21, (6, 5), generator=g)
+    w, dw = torch.rand(2, 6, 5, generator=g)
+    x, dx = torch.randn(2, 4, 9, generator=g)
+    dy, ddy = torch.randn(2, 6, 8, generator=g)
+
+    def tangents(device):
+        def dual(a, b):
+            return fwd.make_dual(a.to(device), b.to(device))
+        i = ids.to(device)
+        with fwd.dual_level():
+            out = [embed_tokens(dual(T, dT), i, 2.0),
+                   sum_tokens(dual(T, dT), i, w.to(device), 0.5),
+                   sum_tokens(T.to(device), i, dual(w, dw)),
+                   token_table_grad(dual(dy, ddy), i, 20, w.to(device)),
+                   token_table_grad(dy.to(device), i, 20, dual(w, dw)),
+                   dropout(dual(x, dx), 0.3, 5, 1)]
+            out = [fwd.unpack_dual(y).tangent for y in out]
+            assert all(t is not None for t in out)
+            return [t.cpu() for t in out]
+
+    # sums of up to ten terms under 20: ten roundings of 2^-24 a side
+    for a, b in zip(tangents("cpu"), tangents("cuda")):
+        assert torch.allclose(a, b, atol=4e-5)
+
+
+def test_sparse_scores_do_not_lose_a_tangent():
+    """torch has no forward mode for CSR rows, and says so."""
+    X = torch.eye(6).to_sparse_csr().cuda()
+    W = torch.ones(6, 2, device="cuda")
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError):
+            csr_matmul(X, fwd.make_dual(W, W))
+
+
+def test_function_transforms():
+    """vmap and jvp hand over tensors without memory of their own."""
+    g = gen(4)
+    x = torch.randn(3, 40, generator=g).cuda()
+    got = torch.func.vmap(lambda a: dropout(a, 0.4, 7, 2))(x)
+    want = torch.stack([dropout(a, 0.4, 7, 2) for a in x])
+    assert torch.allclose(got, want)
+    _, t = torch.func.jvp(lambda a: dropout(a, 0.4, 7, 2), (x,), (x,))
+    assert torch.allclose(t, dropout(x, 0.4, 7, 2))
+
+
 # ------------------------------------------------------------ types, shapes
 def test_gradient_of_a_single_lookup(hip):
     """Ids of no dimension, and rows of no columns."""
