@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 
 from ...parallel.dataset import Dataset, TensorDataset
+from ...utils.derivatives import differentiated
 from ...workflow.pipeline import (BatchTransformer, LabelEstimator,
                                   TupleDataset)
 
@@ -45,7 +46,8 @@ class QuantizedLinearMapper(BatchTransformer):
             self.packed = self.packed.to(X.device)
         if self.b is not None:
             self.b = self.b.to(X.device)
-        if X.is_cuda and hip.gpu_ready():
+        # what the kernel returns has no gradient; torch's rounding passes it on
+        if X.is_cuda and not differentiated(X, self.b) and hip.gpu_ready():
             if X.dtype in (torch.float32, torch.bfloat16, torch.float16):
                 return hip.fp8_linear(X, self.packed, self.b)
             out = hip.fp8_linear(X.to(torch.float32), self.packed, self.b)

@@ -41,6 +41,21 @@ def test_quantized_scores_of_whole_number_features(dtype):
     assert torch.allclose(got.cpu(), want, rtol=0, atol=202 * 2 ** -24 * 6400)
 
 
+def test_quantized_scores_keep_gradients():
+    g = gen(2)
+    q = LinearMapper(torch.randn(300, 5, generator=g)).quantize()
+    X = torch.randn(9, 300, generator=g)
+    grads = []
+    for x in (X.clone().requires_grad_(), X.cuda().requires_grad_()):
+        q.apply_batch(x).square().sum().backward()
+        grads.append(x.grad.cpu())
+    assert grads[0].abs().sum() > 0
+    assert torch.allclose(*grads, rtol=1e-4, atol=1e-4)
+    with fwd.dual_level():
+        x = fwd.make_dual(X.cuda(), torch.ones(9, 300, device="cuda"))
+        assert fwd.unpack_dual(q.apply_batch(x)).tangent is not None
+
+
 # --------------------------------------------------------------- transforms
 def test_tangents_go_through():
     """Forward mode: a dual tensor asks for no gradient in reverse, and its
