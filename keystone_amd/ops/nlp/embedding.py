@@ -60,6 +60,7 @@ def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
         return hip.embedding_bag(table, ids, None, weights, scale)
     rows = embed_tokens(table, ids)
     if weights is not None:
+        weights = weights.masked_fill(~_seen(ids, table.shape[0]), 0.0)
         rows = rows * weights.unsqueeze(-1).to(rows.dtype)
     return rows.sum(1) * scale
 

@@ -4,6 +4,8 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from keystone_amd.ops.nlp.embedding import (embed_tokens, sum_tokens,
+                                            token_table_grad)
 from keystone_amd.utils.derivatives import differentiated
 
 
@@ -25,3 +27,20 @@ def test_what_counts_as_differentiated():
     with fwd.dual_level():
         assert differentiated(fwd.make_dual(x, x)) and not differentiated(x)
     assert not differentiated(x)
+
+
+def test_absent_words_weigh_nothing():
+    """A word outside the table is no term of a sum whatever its weight, and
+    has no gradient."""
+    T = torch.randn(4, 3, requires_grad=True)
+    ids = torch.tensor([[0, -1, 3], [4, -1, -1]])
+    for bad in (float("nan"), float("inf")):
+        w = torch.tensor([[2.0, bad, 1.0], [bad, bad, bad]], requires_grad=True)
+        y = sum_tokens(T, ids, w)
+        assert torch.equal(y[0], 2 * T[0] + T[3]) and y[1].eq(0).all()
+        dT, dw = torch.autograd.grad(y.sum(), (T, w))
+        want = torch.zeros(4, 3)
+        want[0], want[3] = 2, 1
+        assert torch.equal(dT, want) and dw[1].eq(0).all() and dw[0, 1] == 0
+        assert torch.equal(token_table_grad(torch.ones(2, 3), ids, 4, w.detach()),
+                           want)
