@@ -38,12 +38,28 @@ def _seen(ids: torch.Tensor, rows: int) -> torch.Tensor:
     return (ids >= 0) & (ids < rows)
 
 
+def _kernel_ids(ids: torch.Tensor) -> torch.Tensor:
+    """Ids in one of the kernels' two types."""
+    if ids.dtype in (torch.int32, torch.int64) or ids.is_floating_point():
+        return ids
+    return ids.long()
+
+
+def _kernel_weights(weights: Optional[torch.Tensor]):
+    return None if weights is None else weights.to(torch.float32)
+
+
+def _wide(dtype: torch.dtype) -> torch.dtype:
+    """What sums are held in: 32 bits or more."""
+    return torch.promote_types(dtype, torch.float32)
+
+
 def embed_tokens(table: torch.Tensor, ids: torch.Tensor,
                  scale: float = 1.0) -> torch.Tensor:
     """``scale * table[ids]``, [*ids.shape, D]."""
     hip = _hip(table, ids)
     if hip is not None:
-        return hip.embedding_lookup(table, ids, scale)
+        return hip.embedding_lookup(table, _kernel_ids(ids), scale)
     seen = _seen(ids, table.shape[0])
     out = table.new_zeros(*ids.shape, table.shape[1])
     out[seen] = table[ids[seen].long()] * scale
@@ -54,35 +70,41 @@ def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
                weights: Optional[torch.Tensor] = None,
                scale: float = 1.0) -> torch.Tensor:
     """``scale * sum_j weights[b, j] table[ids[b, j]]``, [B, D], of ids
-    [B, L]."""
+    [B, L], in the table's type: rounded once."""
     hip = _hip(table, ids, weights)
     if hip is not None:
-        return hip.embedding_bag(table, ids, None, weights, scale)
-    rows = embed_tokens(table, ids)
+        return hip.embedding_bag(table, _kernel_ids(ids), None,
+                                 _kernel_weights(weights), scale)
+    rows = embed_tokens(table, ids).to(_wide(table.dtype))
     if weights is not None:
         weights = weights.masked_fill(~_seen(ids, table.shape[0]), 0.0)
         rows = rows * weights.unsqueeze(-1).to(rows.dtype)
-    return rows.sum(1) * scale
+    return (rows.sum(1) * scale).to(table.dtype)
 
 
 def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
                      weights: Optional[torch.Tensor] = None,
                      scale: float = 1.0, out: Optional[torch.Tensor] = None
                      ) -> torch.Tensor:
-    """``sum_tokens``'s gradient with respect to the table, [num_rows, D];
-    with ``out`` it is added to ``out``."""
+    """``sum_tokens``'s gradient with respect to the table, [num_rows, D] in
+    grad's type; with ``out`` it is added to ``out``."""
     hip = _hip(grad, ids, weights)
-    if hip is not None:
-        plan = hip.embedding_plan(ids, num_rows, pooled=True)
-        return hip.embedding_grad(grad, plan, weights, scale, out=out,
-                                  accumulate=out is not None)
-    g = grad.unsqueeze(1).expand(*ids.shape, grad.shape[1])
+    if hip is not None and (out is None or out.dtype in (
+            torch.float32, torch.bfloat16, torch.float16)):
+        plan = hip.embedding_plan(_kernel_ids(ids), num_rows, pooled=True)
+        return hip.embedding_grad(grad, plan, _kernel_weights(weights), scale,
+                                  out=out, accumulate=out is not None,
+                                  dtype=grad.dtype)
+    wide = _wide(grad.dtype)
+    g = grad.to(wide).unsqueeze(1).expand(*ids.shape, grad.shape[1])
     if weights is not None:
-        g = g * weights.unsqueeze(-1).to(g.dtype)
+        g = g * weights.unsqueeze(-1).to(wide)
     seen = _seen(ids, num_rows)
-    if out is None:
-        out = grad.new_zeros(num_rows, grad.shape[1])
-    return out.index_add_(0, ids[seen].long(), g[seen] * scale)
+    at, g = ids[seen].long(), g[seen] * scale
+    if out is not None and out.dtype == wide:
+        return out.index_add_(0, at, g)
+    sums = g.new_zeros(num_rows, grad.shape[1]).index_add_(0, at, g)
+    return sums.to(grad.dtype) if out is None else out.add_(sums)
 
 
 def mean_weights(ids: torch.Tensor, num_rows: int) -> torch.Tensor:

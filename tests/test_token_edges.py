@@ -4,8 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from keystone_amd.ops.nlp.embedding import (embed_tokens, sum_tokens,
-                                            token_table_grad)
+from keystone_amd.ops.nlp.embedding import sum_tokens, token_table_grad
 from keystone_amd.utils.derivatives import differentiated
 
 
@@ -44,3 +43,25 @@ def test_absent_words_weigh_nothing():
         assert torch.equal(dT, want) and dw[1].eq(0).all() and dw[0, 1] == 0
         assert torch.equal(token_table_grad(torch.ones(2, 3), ids, 4, w.detach()),
                            want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sums_of_16_bit_tables_round_once(dtype):
+    """32 terms of 1 + eps: in 32 bits each partial sum is exact (24 bits, with
+    a weight that bfloat16 cannot hold), and the result rounds once."""
+    one, weight = 1 + torch.finfo(dtype).eps, 1 + 2.0 ** -8
+    T = torch.tensor([[one], [0.25]], dtype=dtype)
+    ids = torch.zeros(2, 32, dtype=torch.int64)
+    ids[1, 16:] = 1
+    w = torch.full((2, 32), weight)
+    exact = torch.tensor([[32 * one], [16 * one + 4]], dtype=torch.float64)
+    assert torch.equal(sum_tokens(T, ids), exact.to(dtype))
+    assert torch.equal(sum_tokens(T, ids, w, 2.0), (exact * 2 * weight).to(dtype))
+    dy = torch.tensor([[one], [0.25]], dtype=dtype)
+    want = torch.tensor([[32 * one + 4], [4.0]], dtype=torch.float64)
+    got = token_table_grad(dy, ids, 2)
+    assert got.dtype == dtype and torch.equal(got, want.to(dtype))
+    for out in (torch.ones(2, 1), torch.ones(2, 1, dtype=dtype),
+                torch.ones(2, 1, dtype=torch.float64)):
+        again = token_table_grad(dy, ids, 2, None, 1.0, out)
+        assert again is out and torch.equal(out, (want + 1).to(out.dtype))

@@ -108,6 +108,32 @@ def test_function_transforms():
 
 
 # ------------------------------------------------------------ types, shapes
+def test_types_that_the_cpu_takes():
+    g = gen(5)
+    T = torch.randn(30, 12, generator=g)
+    ids = torch.randint(-1, 31, (8, 6), generator=g)
+    w = torch.rand(8, 6, generator=g)
+    dy = torch.randn(8, 12, generator=g)
+    for t in TYPES:
+        for wt in (torch.float64, torch.float32, torch.bfloat16, torch.float16):
+            for it in (torch.int64, torch.int32, torch.int16, torch.int8):
+                outs = []
+                for dev in ("cpu", "cuda"):
+                    a, i, v, d = (T.to(t).to(dev), ids.to(it).to(dev),
+                                  w.to(wt).to(dev), dy.to(t).to(dev))
+                    outs.append((embed_tokens(a, i, 1.5), sum_tokens(a, i, v, 0.5),
+                                 token_table_grad(d, i, 30, v, 0.5),
+                                 token_table_grad(d, i, 30, v, 0.5,
+                                                  out=a.clone().float())))
+                for a, b in zip(*outs):
+                    assert a.dtype == b.dtype
+                    # both sides sum in 32 bits and round once; sums of ten
+                    # and fewer terms, whose roundings may fall either way
+                    step = torch.finfo(a.dtype).eps
+                    assert torch.allclose(a.float(), b.cpu().float(),
+                                          rtol=step, atol=1e-5), (t, wt, it)
+
+
 def test_gradient_of_a_single_lookup(hip):
     """Ids of no dimension, and rows of no columns."""
     T = torch.randn(5, 3, device="cuda")
