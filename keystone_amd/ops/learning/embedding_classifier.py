@@ -123,7 +123,7 @@ class EmbeddingClassifierEstimator(LabelEstimator):
         rt.all_reduce_(most, "max")
         steps = self.num_epochs * -(-int(most.item()) // self.batch_size)
         g = torch.Generator().manual_seed(self.seed + 7919 * rt.rank)
-        seed = self.seed + 7919 * rt.rank
+        seed = (self.seed + 7919 * rt.rank) % 2 ** 64
         order, at = torch.empty(0, dtype=torch.int64), 0
         for step in range(steps):
             if at >= order.numel():

@@ -224,7 +224,8 @@ class MiniBatchSGDwithL2(LabelEstimator):
             idx = torch.randperm(n_local, generator=g)[:bs].to(X.device)
             Xb = X[idx]
             if self.dropout:
-                Xb = dropout(Xb, self.dropout, self.seed + 7919 * rt.rank, it)
+                Xb = dropout(Xb, self.dropout,
+                             (self.seed + 7919 * rt.rank) % 2 ** 64, it)
             _loss, grad = self.gradient.compute(W, Xb, Y[idx])
             grad = grad.to(torch.float64)
             rt.all_reduce_(grad)

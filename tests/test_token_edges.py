@@ -4,6 +4,10 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+import keystone_amd as ka
+from keystone_amd.ops.learning import (EmbeddingClassifierEstimator,
+                                       LeastSquaresGradient,
+                                       MiniBatchSGDwithL2)
 from keystone_amd.ops.nlp.embedding import sum_tokens, token_table_grad
 from keystone_amd.utils.derivatives import differentiated
 
@@ -65,3 +69,18 @@ def test_sums_of_16_bit_tables_round_once(dtype):
                 torch.ones(2, 1, dtype=torch.float64)):
         again = token_table_grad(dy, ids, 2, None, 1.0, out)
         assert again is out and torch.equal(out, (want + 1).to(out.dtype))
+
+
+def test_any_seed_that_torch_takes():
+    """Negative seeds too, which torch's generators count modulo 2^64."""
+    ids, y = torch.randint(-1, 9, (20, 4)), torch.randint(0, 3, (20,))
+    X = torch.randn(20, 5)
+    for p in (0.0, 0.3):
+        a, b = (EmbeddingClassifierEstimator(
+            9, 3, dim=4, num_epochs=1, batch_size=8, dropout=p, seed=s).fit(
+            ka.from_rows(ids), ka.from_rows(y)) for s in (-5, 2 ** 64 - 5))
+        assert torch.equal(a.table, b.table) and torch.equal(a.head.W, b.head.W)
+        a, b = (MiniBatchSGDwithL2(LeastSquaresGradient(), 3, seed=s, dropout=p
+                                   ).fit(ka.from_rows(X), ka.from_rows(y)).W
+                for s in (-5, 2 ** 64 - 5))
+        assert torch.equal(a, b)
