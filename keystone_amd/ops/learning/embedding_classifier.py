@@ -112,16 +112,19 @@ class EmbeddingClassifierEstimator(LabelEstimator):
         if y.dim() > 1:
             y = y.argmax(dim=1)
         y = y.to(ids.device).long()
-        if ids.dim() != 2 or ids.shape[0] != y.shape[0]:
-            raise ValueError(f"expected ids [n, L] and labels [n], got "
-                             f"{tuple(ids.shape)} and {tuple(y.shape)}")
-        n = ids.shape[0]
-        if n and not 0 <= int(y.min()) <= int(y.max()) < self.num_classes:
-            raise ValueError(f"expected labels in [0, {self.num_classes})")
-        params = self.initial(ids.device)
-        most = torch.tensor([n], dtype=torch.int64)
+        n, wrong = y.shape[0], None
+        if ids.dim() != 2 or ids.shape[0] != n:
+            wrong = (f"expected ids [n, L] and labels [n], got "
+                     f"{tuple(ids.shape)} and {tuple(y.shape)}")
+        elif n and not 0 <= int(y.min()) <= int(y.max()) < self.num_classes:
+            wrong = f"expected labels in [0, {self.num_classes})"
+        # all ranks refuse what one does: none waits for it in a reduction
+        most = torch.tensor([n, wrong is not None], dtype=torch.int64)
         rt.all_reduce_(most, "max")
-        steps = self.num_epochs * -(-int(most.item()) // self.batch_size)
+        if most[1]:
+            raise ValueError(wrong or "another rank refused its ids or labels")
+        params = self.initial(ids.device)
+        steps = self.num_epochs * -(-int(most[0]) // self.batch_size)
         g = torch.Generator().manual_seed(self.seed + 7919 * rt.rank)
         seed = (self.seed + 7919 * rt.rank) % 2 ** 64
         order, at = torch.empty(0, dtype=torch.int64), 0

@@ -10,6 +10,7 @@ from keystone_amd.ops.learning import (EmbeddingClassifierEstimator,
                                        MiniBatchSGDwithL2)
 from keystone_amd.ops.nlp.embedding import sum_tokens, token_table_grad
 from keystone_amd.utils.derivatives import differentiated
+from tests.dist_util import run_distributed
 
 
 def test_what_counts_as_differentiated():
@@ -84,3 +85,27 @@ def test_any_seed_that_torch_takes():
                                    ).fit(ka.from_rows(X), ka.from_rows(y)).W
                 for s in (-5, 2 ** 64 - 5))
         assert torch.equal(a, b)
+
+
+def _fit_refused(rank, world, wrong):
+    ids, y = torch.zeros(6, 3, dtype=torch.int64), torch.zeros(6, dtype=torch.int64)
+    if rank == 1 and wrong == "label":
+        y[4] = 7
+    elif rank == 1 and wrong == "rows":
+        y = y[:5]
+    elif rank == 1:
+        ids = ids[:, 0]
+    try:
+        EmbeddingClassifierEstimator(9, 3, dim=4, num_epochs=1).fit(
+            ka.from_rows(ids), ka.from_rows(y))
+    except ValueError as e:
+        return str(e)
+    return "fitted"
+
+
+@pytest.mark.parametrize("wrong,says", [("label", "labels in"), ("rows", "ids"),
+                                        ("ids", "ids")])
+def test_what_one_rank_refuses_all_ranks_refuse(wrong, says):
+    """Or the others would wait for it in the first reduction."""
+    other, own = run_distributed(_fit_refused, 2, (wrong,))
+    assert says in own and "rank" in other
