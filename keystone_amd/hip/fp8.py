@@ -24,6 +24,12 @@ _MAX = 2 ** 31 - 2048      # rows
 _MAX_INNER = 2 ** 26
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Whole and from 16 bytes on, as the kernels read it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 class Fp8Weight:
     """``W`` [K, N] in 8 bits, laid out as the matrix instruction reads it:
     ``data`` [N/16, K/128, 2048] bytes and ``scales`` [N/16, K/512, 64]
@@ -38,7 +44,7 @@ class Fp8Weight:
                 raise ValueError(f"Fp8Weight: expected uint8 {shape} for W "
                                  f"[{K}, {N}], got {t.dtype} "
                                  f"{tuple(t.shape)}")
-        self.data, self.scales = data.contiguous(), scales.contiguous()
+        self.data, self.scales = _aligned(data), _aligned(scales)
         self.K, self.N = K, N
 
     def to(self, device) -> "Fp8Weight":

@@ -5,6 +5,7 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 import keystone_amd as ka
+from keystone_amd import hip
 from keystone_amd.ops.learning import (EmbeddingClassifierEstimator,
                                        LeastSquaresGradient,
                                        MiniBatchSGDwithL2)
@@ -109,3 +110,21 @@ def test_what_one_rank_refuses_all_ranks_refuse(wrong, says):
     """Or the others would wait for it in the first reduction."""
     other, own = run_distributed(_fit_refused, 2, (wrong,))
     assert says in own and "rank" in other
+
+
+@pytest.mark.parametrize("off", [1, 4, 8])
+def test_packed_weights_from_views_are_aligned(off):
+    """The kernels read them 16 bytes at a time; bytes taken out of a larger
+    buffer need not lie so."""
+    W = hip.fp8_pack(torch.randn(300, 40))
+
+    def moved(t):
+        flat = torch.zeros(t.numel() + 64, dtype=torch.uint8)
+        at = flat[(off - flat.data_ptr()) % 16:][:t.numel()].view(t.shape)
+        at.copy_(t)
+        assert at.data_ptr() % 16 == off
+        return at
+
+    again = hip.Fp8Weight(moved(W.data), moved(W.scales), 300, 40)
+    for a, b in ((again.data, W.data), (again.scales, W.scales)):
+        assert a.data_ptr() % 16 == 0 and torch.equal(a, b)

@@ -56,6 +56,21 @@ def test_quantized_scores_keep_gradients():
         assert fwd.unpack_dual(q.apply_batch(x)).tangent is not None
 
 
+@pytest.mark.parametrize("M,K,N", [(3, 2000, 40), (1100, 2300, 40),
+                                   (2100, 2176, 1030)])
+def test_packed_weights_from_a_larger_buffer(hip, M, K, N):
+    g = gen(K)
+    W = hip.fp8_pack(torch.randn(K, N, generator=g).cuda())
+    X = torch.randn(M, K, generator=g).cuda()
+    buffer = torch.cat([torch.zeros(5, dtype=torch.uint8, device="cuda"),
+                        W.data.reshape(-1), W.scales.reshape(-1)])
+    data = buffer[5:5 + W.data.numel()].view(W.data.shape)
+    again = hip.Fp8Weight(data, buffer[5 + W.data.numel():].view(W.scales.shape),
+                          K, N)
+    for x in (X, X.to(torch.bfloat16)):
+        assert torch.equal(hip.fp8_linear(x, again), hip.fp8_linear(x, W))
+
+
 # --------------------------------------------------------------- transforms
 def test_tangents_go_through():
     """Forward mode: a dual tensor asks for no gradient in reverse, and its
