@@ -791,15 +791,22 @@ template <typename T, int VEC>
 int lookup(const Ids& ids, long long n, const void* src, long long ld,
            void* out, int D, float scale, hipStream_t stream) {
     const unsigned cols = (D + VEC - 1) / VEC;
-    const long long vectors = n * cols;
     const unsigned magic = cols == 1 || cols > 32768
                                ? 0 : (unsigned)((1ull << 32) / cols) + 1;
     // 268 MB of rows past the caches leave the table there: 55 us against 88;
     // what fits the caches is left there for its reader
     auto* kernel = n * D * (long long)sizeof(T) >= LARGE
                        ? lookup_kernel<T, VEC, true> : lookup_kernel<T, VEC, false>;
-    kernel<<<(unsigned)((vectors + 1023) / 1024), 256, 0, stream>>>(
-        ids, vectors, (const T*)src, ld, (T*)out, D, cols, magic, scale);
+    // a launch has fewer than 2^32 threads, a quarter of its vectors
+    const long long most = (1ll << 33) / cols;
+    for (long long at = 0; at < n; at += most) {
+        const long long vectors = (n - at < most ? n - at : most) * cols;
+        const Ids some{(const char*)ids.p + at * (ids.wide ? 8 : 4), ids.wide,
+                       ids.rows};
+        kernel<<<(unsigned)((vectors + 1023) / 1024), 256, 0, stream>>>(
+            some, vectors, (const T*)src, ld, (T*)out + at * D, D, cols, magic,
+            scale);
+    }
     return (int)hipGetLastError();
 }
 

@@ -163,3 +163,23 @@ def test_gradient_of_a_single_lookup(hip):
     y = hip.embedding_lookup(T[:, :0], ids)
     assert y.shape == (2, 4, 0)
     assert hip.embedding_grad(y, hip.embedding_plan(ids, 5)).shape == (5, 0)
+
+
+# -------------------------------------------------------------- large sizes
+def test_more_ids_than_a_launch_takes(hip):
+    """2^32 threads of a launch are 2^34 rows of one column."""
+    n = 2 ** 34 + 37
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    T = torch.tensor([[1.0], [2.0], [3.0]], device="cuda").to(torch.bfloat16)
+    at = torch.tensor([0, 2 ** 31, 2 ** 33 - 1, 2 ** 33, 2 ** 33 + 1, 2 ** 34 - 1,
+                       2 ** 34, 2 ** 34 + 36], device="cuda")
+    ids[at] = torch.tensor([2, 1, 2, 1, -1, 2, 1, 2], dtype=torch.int32,
+                           device="cuda")
+    got = hip.embedding_lookup(T, ids)
+    assert got[at, 0].tolist() == [3, 2, 3, 2, 0, 3, 2, 3]
+    for p in at[1:].tolist():
+        near = got[p - 200:p + 36, 0]
+        assert near.eq(1).sum() >= near.numel() - 4 and near.ne(0).sum() >= \
+            near.numel() - 1
+    del ids, got, near
+    torch.cuda.empty_cache()
