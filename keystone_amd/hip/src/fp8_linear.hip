@@ -122,10 +122,11 @@ __device__ __forceinline__ int quantise_block(const float (&v)[4][8],
 template <typename T>
 __global__ __launch_bounds__(256)
 void fp8_quantise_kernel(const T* __restrict__ x, long long ld, int rows,
-                         int K, int tiles, int kblocks,
+                         int K, int tiles, int kblocks, long long first,
                          unsigned char* __restrict__ q,
                          unsigned char* __restrict__ scales) {
-    const long long chunk = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long chunk =
+        first + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (chunk >= (long long)tiles * kblocks) return;
     const int kb = (int)(chunk % kblocks), tile = (int)(chunk / kblocks);
     const int lane = threadIdx.x & 63;
@@ -733,8 +734,12 @@ int quantise(const void* x, long long ld, int rows, int K, unsigned char* q,
              unsigned char* scales, hipStream_t stream) {
     const int tiles = ks_ceil_div(rows, 16), kblocks = ks_ceil_div(K, 128);
     const long long chunks = (long long)tiles * kblocks;
-    fp8_quantise_kernel<T><<<(unsigned)((chunks + 3) / 4), 256, 0, stream>>>(
-        (const T*)x, ld, rows, K, tiles, kblocks, q, scales);
+    // a launch has fewer than 2^32 threads, 64 a chunk
+    const long long most = 1 << 25;
+    for (long long at = 0; at < chunks; at += most)
+        fp8_quantise_kernel<T><<<
+            (unsigned)(((chunks - at < most ? chunks - at : most) + 3) / 4), 256,
+            0, stream>>>((const T*)x, ld, rows, K, tiles, kblocks, at, q, scales);
     return (int)hipGetLastError();
 }
 

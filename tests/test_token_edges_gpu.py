@@ -183,3 +183,18 @@ def test_more_ids_than_a_launch_takes(hip):
             near.numel() - 1
     del ids, got, near
     torch.cuda.empty_cache()
+
+
+def test_more_columns_of_weights_than_a_launch_takes(hip):
+    """2^32 threads of a launch are 2^26 chunks of 16 columns, 137 GB."""
+    N = 2 ** 30 + 21
+    W = torch.randn(1, N, device="cuda", dtype=torch.bfloat16)
+    packed = hip.fp8_pack(W)
+    got = hip.fp8_linear(torch.ones(2, 1, device="cuda", dtype=torch.bfloat16),
+                         packed)
+    for a, b in ((0, 100), (2 ** 29 - 50, 2 ** 29 + 50), (2 ** 30 - 50, N)):
+        want = hip.fp8_round(W[:, a:b].t().float()).t()
+        # one product, whose four bits bfloat16 holds
+        assert torch.equal(got[:, a:b].float(), want.expand(2, -1))
+    del W, packed, got
+    torch.cuda.empty_cache()
