@@ -214,11 +214,29 @@ __device__ __forceinline__ void store_columns(T* y, long long ld, int m, int n,
     }
 }
 
+// An accumulator of mfma_here: read by an instruction that keeps its place, as
+// those of mfma_here do, so that none is moved in front of the wait between them.
+__device__ __forceinline__ f32x4 read_here(const f32x4& acc) {
+    f32x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float x;
+        asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(acc[k]));
+        v[k] = x;
+    }
+    return v;
+}
+
 // A wave's tiles: column n + 16 j, row m + 16 i of y, or of `part` in 32 bits.
-template <typename T, int TM, int TN>
+// HERE: they come from mfma_here.
+template <typename T, int TM, int TN, bool HERE = false>
 __device__ __forceinline__ void store_tiles(const f32x4 (&acc)[TM][TN], T* y,
                                             float* part, const float* bias,
                                             int m, int n, int M, int N) {
+    const auto at_tile = [&](int i, int j) {
+        if constexpr (HERE) return read_here(acc[i][j]);
+        else return acc[i][j];
+    };
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
         const int at = n + j * 16;
@@ -227,13 +245,13 @@ __device__ __forceinline__ void store_tiles(const f32x4 (&acc)[TM][TN], T* y,
 #pragma unroll
             for (int i = 0; i < TM; ++i)
                 if (m + i * 16 < M)
-                    store_columns<float>(part, N, m + i * 16, at, N, acc[i][j]);
+                    store_columns<float>(part, N, m + i * 16, at, N, at_tile(i, j));
         } else {
             const f32x4 b = bias_at(bias, at, N);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
                 if (m + i * 16 < M)
-                    store_columns<T>(y, N, m + i * 16, at, N, acc[i][j] + b);
+                    store_columns<T>(y, N, m + i * 16, at, N, at_tile(i, j) + b);
         }
     }
 }
@@ -510,41 +528,43 @@ constexpr int BIG = 256, STAGES = 4;
 
 // acc += w x^T with byte Q of the scales.  As inline assembly, for its place
 // among the loads: the compiler, to which the two are unrelated, gathers the
-// loads in front and runs out of registers.  Its result is next read as an
-// addend, 64 instructions on, or behind the kernel's own wait at the end.
+// loads in front and runs out of registers.  What the compiler knows of waits does
+// not hold here: an operand that a vector instruction writes just before is seen
+// two cycles later (s_nop 1, while the unit is still at the instruction before:
+// 8192 x 65536 x 1000 bf16 takes 752 us with them and 747 without, f32 1269 and
+// 1268), and a result is read as an addend 64 instructions on, or by read_here
+// behind the kernel's wait.
 template <int Q>
 __device__ __forceinline__ void mfma_here(f32x4& acc, const i32x8& w,
                                           const i32x8& x, unsigned ws,
                                           unsigned xs) {
     if constexpr (Q == 0)
-        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        asm volatile("s_nop 1\n\t"
+                     "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                      "op_sel:[0,0,0] op_sel_hi:[0,0,0]"
                      : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
     else if constexpr (Q == 1)
-        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        asm volatile("s_nop 1\n\t"
+                     "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                      "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
                      : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
     else if constexpr (Q == 2)
-        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        asm volatile("s_nop 1\n\t"
+                     "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                      "op_sel:[0,0,0] op_sel_hi:[1,1,0]"
                      : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
     else
-        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
+        asm volatile("s_nop 1\n\t"
+                     "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                      "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
                      : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs) : "memory");
 }
 
-// The same in bfloat16.  WAIT: an operand may just have been widened, which the
-// matrix unit sees two cycles later.
-template <bool WAIT>
+// The same in bfloat16.
 __device__ __forceinline__ void mfma_here(f32x4& acc, const bf16x8& w,
                                           const bf16x8& x) {
-    if constexpr (WAIT)
-        asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
-                     : "+a"(acc) : "v"(w), "v"(x) : "memory");
-    else
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
-                     : "+a"(acc) : "v"(w), "v"(x) : "memory");
+    asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"
+                 : "+a"(acc) : "v"(w), "v"(x) : "memory");
 }
 
 // What is made of v from here on is made here: the compiler would widen all of
@@ -672,14 +692,9 @@ void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
                 for (int i = 0; i < 8; ++i) {
                     not_before(x[i]);
                     const bf16x8 v = widen(x[i][2 * s], x[i][2 * s + 1], xk[i]);
-                    mfma_here<true>(acc[i][0], wide[0], v);
 #pragma unroll
-                    for (int j = 1; j < 8; ++j) {
-                        if (i == 0)
-                            mfma_here<true>(acc[i][j], wide[j], v);
-                        else
-                            mfma_here<false>(acc[i][j], wide[j], v);
-                    }
+                    for (int j = 0; j < 8; ++j)
+                        mfma_here(acc[i][j], wide[j], v);
                     if (s == 3) x[i] = fetch_x(i, kb + 1);
                 }
                 if (s == 1) arrive();
@@ -709,9 +724,9 @@ void fp8_gemm_big_kernel(Gemm a, T* __restrict__ y, float* __restrict__ part,
             ws[i] = wn[i] & kept(kb + 4);
         }
     }
-    // the last matrix instructions have written their registers
+    // the last matrix instructions have written their registers; see read_here
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    store_tiles<T, 8, 8>(
+    store_tiles<T, 8, 8, true>(
         acc, y, part ? part + (long long)split * a.M * a.N : nullptr, bias,
         m0 * 16 + (lane & 15), n0 * 16 + (lane >> 4) * 4, a.M, a.N);
 }
