@@ -66,18 +66,9 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
 template <typename T, int N, bool PAST>
 __device__ __forceinline__ Vec<T, N> load_buffer(__amdgpu_buffer_rsrc_t b,
                                                  unsigned at) {
-    constexpr int BYTES = N * sizeof(T), NT = PAST ? 2 : 0;
-    if constexpr (BYTES == 16)
-        return __builtin_bit_cast(
-            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, NT));
-    else if constexpr (BYTES == 8)
-        return __builtin_bit_cast(
-            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, NT));
-    else if constexpr (BYTES == 4)
-        return __builtin_bit_cast(
-            Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, NT));
-    else
-        return Vec<T, N>{};       // not reached: a row of eight lanes is longer
+    static_assert(N * sizeof(T) == 16);
+    return __builtin_bit_cast(
+        Vec<T, N>, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, PAST ? 2 : 0));
 }
 
 // Where lane c of a row begins: at c VEC, the last one early enough to end with
@@ -415,22 +406,41 @@ struct Sum {
     Cut c;
 };
 
+// Rows of eight lanes or more have 16 bytes a lane; shorter reads are for rows of
+// one lane or two.
+template <typename TS, int VEC>
+constexpr bool WHOLE = VEC * sizeof(TS) == 16;
+
+// Sums entries [b, e) by teams of 2^el_log groups of lanes: by one of them, or by
+// `waves` of a wave each.  el: the lane's group among the el_n of all of them.
+template <typename TS, typename TO, int VEC, bool ONCE>
+__device__ __forceinline__ void add_rows(const Sum<TS, TO>& a, int col, bool live,
+                                         int b, int e, int el_log, int wave,
+                                         int waves, int el, int el_n,
+                                         float (&acc)[VEC]) {
+    if constexpr (WHOLE<TS, VEC>) {
+        if (a.c.bytes) {
+            add_buffered<TS, VEC, ONCE>(a.t, a.src, a.c.bytes, a.c.pitch, col, b, e,
+                                        a.c.g_log, el_log, wave, waves, acc);
+            return;
+        }
+        if (a.c.pitch) {
+            add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live,
+                                       b, e, a.c.g_log, el_log, wave, waves, acc);
+            return;
+        }
+    }
+    add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, b, e, el, el_n, acc);
+}
+
 // Sums entries [b, e) by the whole block.
 template <typename TS, typename TO, int VEC, bool ONCE>
 __device__ __forceinline__ void add_by_block(const Sum<TS, TO>& a, int col,
                                              bool live, int b, int e,
                                              float (&acc)[VEC]) {
-    if (a.c.bytes)
-        add_buffered<TS, VEC, ONCE>(a.t, a.src, a.c.bytes, a.c.pitch, col, b, e,
-                                    a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6, 4,
-                                    acc);
-    else if (a.c.pitch)
-        add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live, b,
-                                   e, a.c.g_log, 6 - a.c.g_log, threadIdx.x >> 6,
-                                   4, acc);
-    else
-        add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, b, e,
-                             threadIdx.x >> a.c.g_log, 256 >> a.c.g_log, acc);
+    add_rows<TS, TO, VEC, ONCE>(a, col, live, b, e, 6 - a.c.g_log,
+                                threadIdx.x >> 6, 4, threadIdx.x >> a.c.g_log,
+                                256 >> a.c.g_log, acc);
 }
 
 // The long segment that entry i lies in, else -1; a whole wave's work.
@@ -546,17 +556,8 @@ void segment_sum_kernel(Sum<TS, TO> a) {
     }
     for (int k = threadIdx.x >> team_log; k < teams_share; k += 256 >> team_log) {
         float acc[VEC] = {};
-        if (a.c.bytes)
-            add_buffered<TS, VEC, ONCE>(a.t, a.src, a.c.bytes, a.c.pitch, col,
-                                        from[k], to[k], a.c.g_log, a.c.el_log, 0,
-                                        1, acc);
-        else if (a.c.pitch)
-            add_batches<TS, VEC, ONCE>(a.t, a.src, a.c.pitch, a.c.unit, col, live,
-                                       from[k], to[k], a.c.g_log, a.c.el_log, 0,
-                                       1, acc);
-        else
-            add_entries<TS, VEC>(a.t, a.src, a.ld, col, live, from[k], to[k],
-                                 el, el_n, acc);
+        add_rows<TS, TO, VEC, ONCE>(a, col, live, from[k], to[k], a.c.el_log, 0, 1,
+                                    el, el_n, acc);
         add_lanes<VEC>(acc, g_n, g_n * el_n);
         if (live && el == 0)
             put_row<TO, VEC>(a.out + (long long)seg[k] * a.ldo + col, acc,
@@ -699,7 +700,8 @@ int segment_sum(const SumCall& a) {
     c.unit = 0;
     while (c.unit < 6 && a.ld && !(a.ld >> c.unit & 1)) ++c.unit;
     const long long pitch = a.ld >> c.unit;
-    c.pitch = c.g_log >= 3 && pitch * a.t.ids.rows < 0xffffffffll
+    c.pitch = WHOLE<TS, VEC> && c.g_log >= 3 &&
+                      pitch * a.t.ids.rows < 0xffffffffll
                   ? (unsigned)pitch : 0;
     // through a buffer: up to 2 GB, at whole words
     const long long bytes =
@@ -753,11 +755,13 @@ int segment_sum(const SumCall& a) {
     // 149 us with the writes past them, 137 us with the reads too.
     const int past = !a.accumulate &&
                      (long long)a.segs.count * a.D * sizeof(TO) >= LARGE;
-    const bool once = a.once && (long long)a.segs.n * a.D * sizeof(TS) >= LARGE;
+    const bool once = c.pitch && a.once &&
+                      (long long)a.segs.n * a.D * sizeof(TS) >= LARGE;
     const Sum<TS, TO> s{a.segs, a.t, (const TS*)a.src, a.ld, (TO*)a.out, a.ldo,
                         a.D, a.scale, a.accumulate, past, c};
-    auto* kernel = once ? segment_sum_kernel<TS, TO, VEC, true>
-                        : segment_sum_kernel<TS, TO, VEC, false>;
+    auto* kernel = segment_sum_kernel<TS, TO, VEC, false>;
+    if constexpr (WHOLE<TS, VEC>)
+        if (once) kernel = segment_sum_kernel<TS, TO, VEC, true>;
     kernel<<<dim3((unsigned)blocks, slices), 256, 0, a.stream>>>(s);
     if (c.chunks)
         segment_join_kernel<TO, VEC><<<dim3(c.chunks, slices), 256, 0,
