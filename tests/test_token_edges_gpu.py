@@ -198,3 +198,100 @@ def test_more_columns_of_weights_than_a_launch_takes(hip):
         assert torch.equal(got[:, a:b].float(), want.expand(2, -1))
     del W, packed, got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [1001, 1024])
+@pytest.mark.parametrize("over", [-1, 1])
+def test_lookup_at_the_cache_border(hip, dtype, D, over):
+    """Just under and just over 32 MB of output, stored through and past the
+    caches; an odd D lets neighbouring lanes write the same elements."""
+    size = torch.finfo(dtype).bits // 8
+    n = (32 << 20) // (D * size) + over
+    g = gen(D + over)
+    T = torch.randn(3001, D, generator=g).to(dtype).cuda()
+    ids = some_ids(n, 3001, g)
+    ok = (ids >= 0) & (ids < 3001)
+    for scale in (1.0, 2.0):
+        want = T[ids.clamp(0, 3000)] * scale
+        want[~ok] = 0
+        assert torch.equal(hip.embedding_lookup(T, ids, scale), want)
+
+
+@pytest.mark.parametrize("src", TYPES)
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("D,over", [(1001, -1), (1001, 1), (512, 1)])
+def test_gradient_at_the_cache_border(hip, src, out, D, over):
+    """Just under and just over 32 MB of gradients that are read once, onto just
+    under and just over 32 MB of sums."""
+    n = (32 << 20) // (D * (torch.finfo(src).bits // 8)) + 1 + over
+    V = (32 << 20) // (D * (torch.finfo(out).bits // 8)) + over
+    g = gen(D + over)
+    ids = some_ids(n, V, g, hot=0.05)
+    dy = torch.randn(n, D, generator=g).to(src).cuda()
+    got = hip.embedding_grad(dy, hip.embedding_plan(ids, V), scale=0.5, dtype=out)
+    check(got, *sums64(dy, torch.arange(n), ids, None, V, 0.5))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,hot", [(900, 1), (900, 600), (5000, 9), (5000, 600),
+                                   (20000, 1), (20000, 5000), (20000, 20000)])
+@pytest.mark.parametrize("D", [1, 37, 130])
+def test_in_place_step_of_a_large_table(hip, dtype, n, hot, D):
+    """Fewer tokens than table rows, one of them `hot` times: rows that do not
+    occur keep their bits, those that do are off by their sum's roundings."""
+    V, g = 50000, gen(n + hot + D)
+    ids = torch.randint(0, V, (n,), generator=g)
+    ids[torch.randperm(n, generator=g)[:hot]] = V // 3
+    dy = torch.randn(n, D, generator=g).to(dtype).cuda()
+    flat = torch.randn(V, D + 9, generator=g).to(dtype).cuda()
+    table, before = flat[:, 3:3 + D], flat.clone()
+    hip.embedding_grad(dy, hip.embedding_plan(ids.cuda(), V), scale=-0.25,
+                       out=table, accumulate=True)
+    want, mag, m = sums64(dy, torch.arange(n), ids, None, V, -0.25)
+    old = before[:, 3:3 + D].cpu().double()
+    seen = torch.zeros(V, dtype=torch.bool)
+    seen[ids] = True
+    check(table.cpu()[seen], (want + old)[seen], (mag + old.abs())[seen],
+          m[seen] + 2)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    a, b = flat.cpu().view(bits), before.cpu().view(bits)
+    assert torch.equal(a[~seen], b[~seen])
+    assert torch.equal(a[:, :3], b[:, :3]) and torch.equal(a[:, 3 + D:], b[:, 3 + D:])
+
+
+@pytest.mark.parametrize("src", TYPES)
+@pytest.mark.parametrize("D", [1, 33, 256])
+def test_weighted_bag_gradient(hip, src, D):
+    lens = [3, 1000, 0, 0, 130, 2, 4000, 7] + [11] * 300
+    n, V, g = sum(lens), 61, gen(D)
+    ids, offsets = some_ids(n, V, g), some_offsets(lens)
+    w = torch.randn(n, generator=g).cuda()
+    dy = torch.randn(len(lens), D, generator=g).to(src).cuda()
+    bag = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+    for out in TYPES:
+        got = hip.embedding_grad(dy, hip.embedding_plan(ids, V, offsets), w, 1.5,
+                                 dtype=out)
+        check(got, *sums64(dy, bag, ids, w, V, 1.5))
+
+
+@pytest.mark.parametrize("D", [1024, 1025, 1030])
+def test_bags_of_a_table_over_32_bit_places(hip, D):
+    """Over 2^31 elements: rows read through 64-bit offsets, in units that a
+    row's length allows, or one by one where it allows none."""
+    V, g = 2 ** 22 + 3, gen(D)
+    rows = torch.tensor([0, 5, V // 2, V - 2, V - 1])
+    table = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    table[rows.cuda()] = torch.randn(5, D, generator=g).to(torch.bfloat16).cuda()
+    lens = [3, 0, 700, 1, 5000, 40]
+    n = sum(lens)
+    ids = rows[torch.randint(0, 5, (n,), generator=g)]
+    ids[::9] = V
+    w = torch.randn(n, generator=g).cuda()
+    got = hip.embedding_bag(table, ids.cuda(), some_offsets(lens), w, 0.5)
+    few = torch.searchsorted(rows, ids)
+    few[ids == V] = -1
+    bag = torch.repeat_interleave(torch.arange(6), torch.tensor(lens))
+    check(got, *sums64(table[rows.cuda()], few, bag, w, 6, 0.5))
+    del table
+    torch.cuda.empty_cache()
