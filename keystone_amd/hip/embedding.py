@@ -185,6 +185,12 @@ class EmbeddingPlan:
         # keys, order, rows where there are bags, starts: one allocation
         self._kept, self._bagged = kept, bagged
 
+    def record_stream(self, stream) -> None:
+        """As ``torch.Tensor.record_stream``: a plan that is used on another
+        stream than the one it was made on and let go of meanwhile keeps its
+        memory until that stream is past here."""
+        self._kept.record_stream(stream)
+
     def _places(self):
         """Where keys, order, rows and starts lie."""
         at, step = self._kept.data_ptr(), 4 * self.n

@@ -165,6 +165,28 @@ def test_gradient_of_a_single_lookup(hip):
     assert hip.embedding_grad(y, hip.embedding_plan(ids, 5)).shape == (5, 0)
 
 
+def test_a_plan_used_on_another_stream_keeps_its_memory(hip):
+    g = gen(9)
+    ids, dy = some_ids(40000, 900, g), torch.randn(40000, 16, generator=g).cuda()
+    plan = hip.embedding_plan(ids, 900)
+    want = hip.embedding_grad(dy, plan)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(10 ** 8)
+        got = hip.embedding_grad(dy, plan)
+    plan.record_stream(other)
+    dy.record_stream(other)
+    at, size = plan.keys.data_ptr(), plan._kept.numel()
+    del plan
+    # what is freed on this stream would be handed out again at once
+    others = [torch.empty(size, dtype=torch.int32, device="cuda")
+              for _ in range(3)]
+    assert all(t.data_ptr() != at for t in others)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 # -------------------------------------------------------------- large sizes
 def test_more_ids_than_a_launch_takes(hip):
     """2^32 threads of a launch are 2^34 rows of one column."""
