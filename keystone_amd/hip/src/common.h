@@ -10,6 +10,13 @@
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// N neighbours in memory, at any element: rows of odd length are read and
+// written 16 bytes at a time like others.
+template <typename T, int N>
+struct InMemory {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
 __host__ __device__ static inline int ks_ceil_div(int a, int b) {
     return (a + b - 1) / b;
 }

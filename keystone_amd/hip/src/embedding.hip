@@ -27,13 +27,6 @@ namespace {
 template <typename T, int N>
 using Vec = T __attribute__((ext_vector_type(N)));
 
-// The same in memory, at any element: rows of odd length are read and written
-// 16 bytes at a time like others.
-template <typename T, int N>
-struct InMemory {
-    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-};
-
 template <typename T, int N, bool PAST = false>
 __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
     using M = typename InMemory<T, N>::type;

@@ -36,12 +36,6 @@ using i32x8 = int __attribute__((ext_vector_type(8)));
 
 constexpr int CHUNK = 2048;
 
-// N neighbours in memory, at any element.
-template <typename T, int N>
-struct InMemory {
-    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-};
-
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
     constexpr int W = 16 / sizeof(T);
@@ -920,12 +914,6 @@ int gemm(const Gemm& a, const Rows<T>& src, void* y, float* part,
     return (int)hipGetLastError();
 }
 
-template <typename T>
-int linear(const Gemm& a, const void* x, long long ld, int K, void* y, float* part,
-           const float* bias, int type, hipStream_t stream) {
-    return gemm<T>(a, Rows<T>{(const T*)x, ld, K}, y, part, bias, type, stream);
-}
-
 // Where a call's workspace has what.
 struct Work {
     bool quantised;    // before the product, in a launch of its own
@@ -984,9 +972,14 @@ KS_EXPORT int ks_fp8_linear(const void* x, int type, long long ld,
                  ks_ceil_div(K, 128)};
     float* part = (float*)(work + w.part);
     switch (type) {
-        case 0: return linear<float>(a, x, ld, K, y, part, bias, type, stream);
-        case 1: return linear<__bf16>(a, x, ld, K, y, part, bias, type, stream);
+        case 0:
+            return gemm<float>(a, {(const float*)x, ld, K}, y, part, bias, type,
+                               stream);
+        case 1:
+            return gemm<__bf16>(a, {(const __bf16*)x, ld, K}, y, part, bias, type,
+                                stream);
         default:
-            return linear<_Float16>(a, x, ld, K, y, part, bias, type, stream);
+            return gemm<_Float16>(a, {(const _Float16*)x, ld, K}, y, part, bias,
+                                  type, stream);
     }
 }
