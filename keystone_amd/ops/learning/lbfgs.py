@@ -94,7 +94,8 @@ class _LBFGSBase(LabelEstimator):
         d = X.shape[1] + (1 if self.fit_intercept else 0)
         # a user's own gradient gets X as the tensor that it is
         if type(self.gradient) in (LeastSquaresGradient, LogisticGradient) \
-                and SparseRows.supports(X):
+                and SparseRows.supports(X) \
+                and not (self.fit_intercept and SparseRows.mostly_filled(X)):
             X = SparseRows(X, self.fit_intercept)
         elif self.fit_intercept:
             ones = torch.ones(X.shape[0], 1, dtype=dtype, device=Y.device)

@@ -54,6 +54,14 @@ class SparseRows:
         return max(*X.shape, X.values().numel()) <= hip.MAX_TOKENS \
             and hip.gpu_ready()
 
+    @staticmethod
+    def mostly_filled(X: torch.Tensor) -> bool:
+        """Whether so many of X's entries are stored that its products are
+        faster dense.  ``X @ W`` and ``X.T @ D`` of 20000 x 20000 by 20
+        columns take 0.57 ms here with 5 in 100 stored, 1.2 ms with 10, and
+        0.70 ms dense; by 147 columns 3.1, 6.1 and 2.7 ms."""
+        return X.values().numel() * 16 > X.shape[0] * X.shape[1]
+
     def __matmul__(self, W: torch.Tensor) -> torch.Tensor:
         S = self.hip.embedding_bag(W[:self.features], self.columns,
                                    self.offsets, self.values)

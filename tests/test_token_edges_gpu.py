@@ -6,8 +6,10 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from keystone_amd.ops.learning import LinearMapper
-from keystone_amd.ops.learning.sparse_rows import csr_matmul
+import keystone_amd as ka
+from keystone_amd.ops.learning import (DenseLBFGSwithL2, LeastSquaresGradient,
+                                       LinearMapper, SparseLBFGSwithL2)
+from keystone_amd.ops.learning.sparse_rows import SparseRows, csr_matmul
 from keystone_amd.ops.nlp.embedding import (embed_tokens, sum_tokens,
                                             token_table_grad)
 from keystone_amd.ops.stats import dropout
@@ -185,6 +187,27 @@ def test_a_plan_used_on_another_stream_keeps_its_memory(hip):
     assert all(t.data_ptr() != at for t in others)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("share,sparse", [(0.03, True), (0.3, False)])
+@pytest.mark.parametrize("intercept", [False, True])
+def test_filled_rows_with_an_intercept_are_fitted_dense(monkeypatch, share,
+                                                        sparse, intercept):
+    """As before there were kernels for CSR rows, which many stored entries make
+    slower; without an intercept those take the place of the library's."""
+    calls, t_matmul = [], SparseRows.t_matmul
+    monkeypatch.setattr(SparseRows, "t_matmul", lambda self, D:
+                        calls.append(1) or t_matmul(self, D))
+    g = gen(10)
+    X = torch.randn(300, 200, generator=g) * (
+        torch.rand(300, 200, generator=g) < share)
+    y = torch.randint(0, 3, (300,), generator=g).cuda()
+    fits = [cls(LeastSquaresGradient(), 1, 1e-3, fit_intercept=intercept).fit(
+        ka.from_rows(A), ka.from_rows(y))
+        for cls, A in ((DenseLBFGSwithL2, X.cuda()),
+                       (SparseLBFGSwithL2, X.to_sparse_csr().cuda()))]
+    assert bool(calls) == (sparse or not intercept)
+    assert torch.allclose(fits[0].W, fits[1].W, rtol=1e-4, atol=1e-6)
 
 
 # -------------------------------------------------------------- large sizes
