@@ -38,10 +38,16 @@ class QuantizedLinearMapper(BatchTransformer):
         return cls(hip.fp8_pack(W), b)
 
     def apply_batch(self, X: torch.Tensor) -> torch.Tensor:
+        if X.dim() < 2 or X.shape[-1] != self.packed.K:
+            raise ValueError(f"QuantizedLinearMapper: rows {tuple(X.shape)} of "
+                             f"features for {self.packed.K} weights")
+        if X.dim() == 2:
+            return self._rows(X)
+        out = self._rows(X.reshape(X.shape[:-1].numel(), X.shape[-1]))
+        return out.reshape(*X.shape[:-1], self.packed.N)
+
+    def _rows(self, X: torch.Tensor) -> torch.Tensor:
         from ... import hip
-        if X.shape[1] != self.packed.K:
-            raise ValueError(f"QuantizedLinearMapper: {X.shape[1]} features "
-                             f"for {self.packed.K} weights")
         if self.packed.data.device != X.device:
             self.packed = self.packed.to(X.device)
         if self.b is not None:

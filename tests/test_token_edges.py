@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as fwd
 import keystone_amd as ka
 from keystone_amd import hip
 from keystone_amd.ops.learning import (EmbeddingClassifierEstimator,
-                                       LeastSquaresGradient,
+                                       LeastSquaresGradient, LinearMapper,
                                        MiniBatchSGDwithL2)
 from keystone_amd.ops.nlp.embedding import sum_tokens, token_table_grad
 from keystone_amd.utils.derivatives import differentiated
@@ -128,3 +128,19 @@ def test_packed_weights_from_views_are_aligned(off):
     again = hip.Fp8Weight(moved(W.data), moved(W.scales), 300, 40)
     for a, b in ((again.data, W.data), (again.scales, W.scales)):
         assert a.data_ptr() % 16 == 0 and torch.equal(a, b)
+
+
+def test_quantized_scores_of_rows_in_several_dimensions():
+    """As LinearMapper and BlockLinearMapper: the last dimension is the
+    features'."""
+    lin = LinearMapper(torch.randn(70, 5), torch.randn(5))
+    q = lin.quantize()
+    for shape in ((2, 70, 70), (3, 4, 70), (0, 4, 70), (2, 0, 70), (1, 1, 1, 70)):
+        X = torch.randn(shape)
+        got = q.apply_batch(X)
+        assert got.shape == lin.apply_batch(X).shape
+        assert torch.equal(got.reshape(-1, 5), q.apply_batch(X.reshape(-1, 70)))
+        ds = ka.from_rows(X)
+        assert torch.equal(q.apply_dataset(ds).data, got)
+    with pytest.raises(ValueError, match="features"):
+        q.apply_batch(torch.randn(2, 70, 71))
