@@ -13,8 +13,8 @@
 //
 // All of it is memory.  Measured on one MI355X (a large copy: 4.75 TB/s):
 //   lookup of 262144 x 512 bf16 rows of 100000: 54 us, 5 TB/s written
-//   sums of 3.3 M f16 rows of 256 over 32768 bags: 127 us, 13 TB/s gathered,
-//     60 % of it from the L2s
+//   sums of 3.3 M f16 rows of 256 over 32768 bags: 127 us, 13 TB/s gathered, 61 %
+//     of it from the L2s, which all hold the same hottest rows
 //   gradient of 1048576 bf16 rows of 256 onto 100000: 136 us, 4.7 TB/s
 //   gradient of 7.8 M weighted entries onto 100000 x 2 f32: 142 us; each
 //     weight, gathered in the sorted order, costs a cache line

@@ -16,13 +16,14 @@
 // past the end and K past the end are zeros.
 //
 // Measured on one MI355X (a large 8-bit library product: 2.66 PFLOP/s):
-//   quantising 8192 x 65536 bf16: 300 us, 5.4 TB/s read and written
-//   8192 x 65536 x 1000 bf16: 456 us with the join, 2.35 PFLOP/s, the matrix
-//     unit 59 % busy
+//   quantising 8192 x 65536 bf16: 289 us, 5.6 TB/s read and written
+//   8192 x 65536 x 1000 bf16: 0.45 to 0.53 ms with the join, 2.0 to 2.35 PFLOP/s
+//     by the clock, the matrix unit 59 % busy
 //   8192 x 65536 x 1000 f32: 845 us, 1.27 PFLOP/s (a large bfloat16 library
 //     product: 1.20)
-//   1 x 16384 x 1000 f32: 7.9 us, 2.1 TB/s of W from 63 blocks
-//   1021 x 8192 x 147 f32: 15.4 us with the join, X at 2.2 TB/s
+//   1 x 16384 x 1000 f32: 8.8 us, 1.9 TB/s of W from 63 blocks
+//   1021 x 8192 x 147 f32: 13.4 us and 3.4 us of the join, X at 2.5 TB/s; it waits
+//     for loads: vector work is a third of its cycles
 //   8192 x 8192 x 10 f32: 52 us, X at 5.2 TB/s
 #include "common.h"
 

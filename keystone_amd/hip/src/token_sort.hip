@@ -11,8 +11,10 @@
 // each one's place is counted instead, in one launch.
 //
 // Bound by latency and launches, tokens of 100000: 777 take 4.7 us, 4096 take
-// 8.2 us, 16384 take 25 us in five launches, 1048576 take 52 us (78 us with
-// scattered writes of 4 bytes), 8388608 take 175 us.
+// 8.2 us, 16384 take 22 us in five launches, 1048576 take 52 us (78 us with
+// scattered writes of 4 bytes), 8388608 take 181 us.  Ids in bags take longer,
+// 7.86 M of them 329 us: the last pass reads a bag's number for each token, and a
+// cache line for it.
 #include "common.h"
 
 #include <cstdint>
