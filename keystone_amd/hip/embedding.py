@@ -157,6 +157,10 @@ def embedding_bag(table: torch.Tensor, ids: torch.Tensor,
     if n > MAX_TOKENS or bags > MAX_TOKENS:
         raise ValueError(f"embedding_bag: {n} ids in {bags} bags are over "
                          f"{MAX_TOKENS}")
+    if weights is not None and weights.dim() > 1 \
+            and weights.shape != ids.shape:
+        raise ValueError(f"embedding_bag.weights: {tuple(weights.shape)} for "
+                         f"ids {tuple(ids.shape)}")
     weights = _weights(weights, n, "embedding_bag.weights", table.device)
     V, D = table.shape
     if n == 0:

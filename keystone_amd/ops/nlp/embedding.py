@@ -49,6 +49,13 @@ def _kernel_weights(weights: Optional[torch.Tensor]):
     return None if weights is None else weights.to(torch.float32)
 
 
+def _bag_weights(weights: Optional[torch.Tensor], ids: torch.Tensor):
+    """A weight for each of the ids, that are rows of bags."""
+    if ids.dim() != 2:
+        raise ValueError(f"expected ids [bags, length], got {tuple(ids.shape)}")
+    return None if weights is None else weights.expand(ids.shape)
+
+
 def _wide(dtype: torch.dtype) -> torch.dtype:
     """What sums are held in: 32 bits or more."""
     return torch.promote_types(dtype, torch.float32)
@@ -71,6 +78,7 @@ def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
                scale: float = 1.0) -> torch.Tensor:
     """``scale * sum_j weights[b, j] table[ids[b, j]]``, [B, D], of ids
     [B, L], in the table's type: rounded once."""
+    weights = _bag_weights(weights, ids)
     hip = _hip(table, ids, weights)
     if hip is not None:
         return hip.embedding_bag(table, _kernel_ids(ids), None,
@@ -88,6 +96,7 @@ def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
                      ) -> torch.Tensor:
     """``sum_tokens``'s gradient with respect to the table, [num_rows, D] in
     grad's type; with ``out`` it is added to ``out``."""
+    weights = _bag_weights(weights, ids)
     hip = _hip(grad, ids, weights)
     if hip is not None and (out is None or out.dtype in (
             torch.float32, torch.bfloat16, torch.float16)):

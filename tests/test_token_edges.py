@@ -144,3 +144,27 @@ def test_quantized_scores_of_rows_in_several_dimensions():
         assert torch.equal(q.apply_dataset(ds).data, got)
     with pytest.raises(ValueError, match="features"):
         q.apply_batch(torch.randn(2, 70, 71))
+
+
+def test_weights_have_the_ids_shape_or_are_spread_over_it():
+    T, ids = torch.randn(9, 3), torch.randint(0, 9, (4, 6))
+    w, dy = torch.rand(4, 6), torch.randn(4, 3)
+    for v in (w[:, :1], w[0], w[:1, :1], w):
+        full = v.expand(4, 6)
+        assert torch.equal(sum_tokens(T, ids, v), sum_tokens(T, ids, full))
+        assert torch.equal(token_table_grad(dy, ids, 9, v),
+                           token_table_grad(dy, ids, 9, full))
+    for v in (w.t(), w[:, :5], w.reshape(-1), w[None]):
+        with pytest.raises((ValueError, RuntimeError)):
+            sum_tokens(T, ids, v)
+        with pytest.raises((ValueError, RuntimeError)):
+            token_table_grad(dy, ids, 9, v)
+
+
+def test_bags_of_ids_are_rows():
+    T = torch.randn(9, 3)
+    for ids in (torch.tensor([1, 2]), torch.zeros(2, 2, 2, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="ids"):
+            sum_tokens(T, ids)
+        with pytest.raises(ValueError, match="ids"):
+            token_table_grad(torch.ones(2, 3), ids, 9)

@@ -210,6 +210,31 @@ def test_filled_rows_with_an_intercept_are_fitted_dense(monkeypatch, share,
     assert torch.allclose(fits[0].W, fits[1].W, rtol=1e-4, atol=1e-6)
 
 
+def test_weights_of_bags_have_the_ids_shape(hip):
+    """Weights of another shape with as many elements would go to other ids."""
+    g = gen(11)
+    T, dy = torch.randn(9, 3, generator=g), torch.randn(4, 3, generator=g)
+    ids, w = torch.randint(-1, 9, (4, 6), generator=g), torch.rand(4, 6, generator=g)
+    for v in (w[:, :1], w[0], w[:1, :1], w):
+        # six roundings of sums of six terms under 4, a side
+        assert torch.allclose(sum_tokens(T.cuda(), ids.cuda(), v.cuda()).cpu(),
+                              sum_tokens(T, ids, v), atol=12 * 2 ** -24 * 24)
+        assert torch.allclose(
+            token_table_grad(dy.cuda(), ids.cuda(), 9, v.cuda()).cpu(),
+            token_table_grad(dy, ids, 9, v), atol=48 * 2 ** -24 * 96)
+    for v in (w.t(), w.reshape(-1), w[None]):
+        with pytest.raises((ValueError, RuntimeError)):
+            sum_tokens(T.cuda(), ids.cuda(), v.cuda())
+        with pytest.raises((ValueError, RuntimeError)):
+            token_table_grad(dy.cuda(), ids.cuda(), 9, v.cuda())
+    for v in (w.t(), w[None]):
+        with pytest.raises(ValueError, match="weights"):
+            hip.embedding_bag(T.cuda(), ids.cuda(), weights=v.cuda())
+    assert torch.equal(
+        hip.embedding_bag(T.cuda(), ids.cuda(), weights=w.reshape(-1).cuda()),
+        hip.embedding_bag(T.cuda(), ids.cuda(), weights=w.cuda()))
+
+
 # -------------------------------------------------------------- large sizes
 def test_more_ids_than_a_launch_takes(hip):
     """2^32 threads of a launch are 2^34 rows of one column."""
