@@ -33,7 +33,8 @@ class EmbeddingClassifierModel(BatchTransformer):
     def apply_batch(self, ids: torch.Tensor) -> torch.Tensor:
         self.table = self.table.to(ids.device)
         return self.head.apply_batch(sum_tokens(
-            self.table, ids, mean_weights(ids, self.table.shape[0])))
+            self.table, ids, mean_weights(ids, self.table.shape[0],
+                                          self.table.dtype)))
 
     def quantize(self) -> "EmbeddingClassifierModel":
         """The same model with its class weights in 8 bits."""
@@ -90,7 +91,7 @@ class EmbeddingClassifierEstimator(LabelEstimator):
         gradients [dE, dW, db].  With ``table_rate`` dE is None and
         ``table_rate`` times it is added to E."""
         E, W, b = params
-        w = mean_weights(ids, E.shape[0])
+        w = mean_weights(ids, E.shape[0], E.dtype)
         h = sum_tokens(E, ids, w)
         hd = dropout(h, self.dropout, seed, step)
         S = hd @ W + b

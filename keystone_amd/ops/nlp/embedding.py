@@ -116,11 +116,12 @@ def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
     return sums.to(grad.dtype) if out is None else out.add_(sums)
 
 
-def mean_weights(ids: torch.Tensor, num_rows: int) -> torch.Tensor:
-    """float32 [B, L]: one over the number of row b's words, so that the
-    weighted sum is their mean (zero for a row without any)."""
+def mean_weights(ids: torch.Tensor, num_rows: int,
+                 dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """[B, L] in 32 bits or more: one over the number of row b's words, so that
+    the weighted sum is their mean (zero for a row without any)."""
     n = _seen(ids, num_rows).sum(1, keepdim=True).clamp(min=1)
-    return (1.0 / n.to(torch.float32)).expand(ids.shape).contiguous()
+    return (1.0 / n.to(_wide(dtype))).expand(ids.shape).contiguous()
 
 
 class PadTokens(Transformer):
@@ -175,5 +176,5 @@ class MeanEmbedding(_TableTransformer):
 
     def apply_batch(self, ids: torch.Tensor) -> torch.Tensor:
         table = self._resident(ids)
-        return sum_tokens(table, ids, mean_weights(ids, table.shape[0]),
-                          self.scale)
+        return sum_tokens(table, ids, mean_weights(ids, table.shape[0],
+                                                   table.dtype), self.scale)

@@ -9,6 +9,7 @@ from keystone_amd import hip
 from keystone_amd.ops.learning import (EmbeddingClassifierEstimator,
                                        LeastSquaresGradient, LinearMapper,
                                        MiniBatchSGDwithL2)
+from keystone_amd.ops.nlp import MeanEmbedding
 from keystone_amd.ops.nlp.embedding import sum_tokens, token_table_grad
 from keystone_amd.utils.derivatives import differentiated
 from tests.dist_util import run_distributed
@@ -168,3 +169,19 @@ def test_bags_of_ids_are_rows():
             sum_tokens(T, ids)
         with pytest.raises(ValueError, match="ids"):
             token_table_grad(torch.ones(2, 3), ids, 9)
+
+
+def test_means_of_64_bit_tables_are_in_64_bits():
+    T = torch.randn(5, 4, dtype=torch.float64)
+    ids = torch.tensor([[0, 1, 2, -1, -1], [3, 3, 4, 0, 1], [-1, 9, -1, -1, -1]])
+    want = torch.stack([T[:3].mean(0), T[[3, 3, 4, 0, 1]].mean(0), T[0] * 0])
+    got = MeanEmbedding(T).apply_batch(ids)
+    assert got.dtype == torch.float64
+    assert torch.allclose(got, want, rtol=0, atol=8 * 2.0 ** -53 * 20)
+    est = EmbeddingClassifierEstimator(5, 3, dim=4, dropout=0.0)
+    params = [p.double() for p in est.initial("cpu")]
+    params[0] = T
+    loss, _ = est.gradients(params, ids, torch.tensor([0, 1, 2]), 3, 1, 2)
+    S = want @ params[1] + params[2]
+    ref = torch.nn.functional.cross_entropy(S, torch.tensor([0, 1, 2]))
+    assert abs(loss.item() - ref.item()) < 1e-14
