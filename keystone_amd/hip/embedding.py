@@ -297,9 +297,14 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
             raise RuntimeError("embedding_grad.out: rows must be contiguous "
                                "and apart")
         if out.numel() and grad.numel():
-            (a, b), (c, d) = _span(out), _span(grad)
-            if a < d and c < b:
-                raise ValueError("embedding_grad: out overlaps grad")
+            a, b = _span(out)
+            read = {"grad": _span(grad)}
+            if weights is not None:
+                c = weights.data_ptr()
+                read["weights"] = c, c + 4 * weights.numel()
+            for name, (c, d) in read.items():
+                if a < d and c < b:
+                    raise ValueError(f"embedding_grad: out overlaps {name}")
     if plan.n == 0 or plan.num_bags == 0:
         return out if accumulate else out.zero_()
     keys, order, rows, starts = plan._places()

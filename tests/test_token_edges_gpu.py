@@ -235,6 +235,19 @@ def test_weights_of_bags_have_the_ids_shape(hip):
         hip.embedding_bag(T.cuda(), ids.cuda(), weights=w.cuda()))
 
 
+def test_sums_do_not_land_on_what_is_still_read(hip):
+    flat = torch.ones(64, device="cuda")
+    ids = torch.arange(8, device="cuda") % 4
+    dy, plan = torch.ones(8, 3, device="cuda"), hip.embedding_plan(ids, 4)
+    out = flat[4:16].view(4, 3)
+    for w in (flat[:8], flat[15:23], flat[6:14]):
+        with pytest.raises(ValueError, match="weights"):
+            hip.embedding_grad(dy, plan, w, out=out, accumulate=True)
+    hip.embedding_grad(dy, plan, flat[16:24], out=out, accumulate=True)
+    torch.cuda.synchronize()
+    assert out.eq(3).all() and flat[:4].eq(1).all() and flat[16:].eq(1).all()
+
+
 # -------------------------------------------------------------- large sizes
 def test_more_ids_than_a_launch_takes(hip):
     """2^32 threads of a launch are 2^34 rows of one column."""
