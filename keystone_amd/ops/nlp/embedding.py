@@ -85,6 +85,7 @@ def sum_tokens(table: torch.Tensor, ids: torch.Tensor,
                                  _kernel_weights(weights), scale)
     rows = embed_tokens(table, ids).to(_wide(table.dtype))
     if weights is not None:
+        # an absent word's may be a NaN
         weights = weights.masked_fill(~_seen(ids, table.shape[0]), 0.0)
         rows = rows * weights.unsqueeze(-1).to(rows.dtype)
     return (rows.sum(1) * scale).to(table.dtype)
@@ -106,9 +107,9 @@ def token_table_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int,
                                   dtype=grad.dtype)
     wide = _wide(grad.dtype)
     g = grad.to(wide).unsqueeze(1).expand(*ids.shape, grad.shape[1])
-    if weights is not None:
-        g = g * weights.unsqueeze(-1).to(wide)
     seen = _seen(ids, num_rows)
+    if weights is not None:
+        g = g * weights.masked_fill(~seen, 0.0).unsqueeze(-1).to(wide)
     at, g = ids[seen].long(), g[seen] * scale
     if out is not None and out.dtype == wide:
         return out.index_add_(0, at, g)

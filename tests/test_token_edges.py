@@ -50,6 +50,10 @@ def test_absent_words_weigh_nothing():
         assert torch.equal(dT, want) and dw[1].eq(0).all() and dw[0, 1] == 0
         assert torch.equal(token_table_grad(torch.ones(2, 3), ids, 4, w.detach()),
                            want)
+        # the sum's gradient is linear in the rows' one: its own derivative
+        dy = torch.ones(2, 3, requires_grad=True)
+        d, = torch.autograd.grad(token_table_grad(dy, ids, 4, w.detach()).sum(), dy)
+        assert d[0].eq(3).all() and d[1].eq(0).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
