@@ -248,6 +248,69 @@ def test_sums_do_not_land_on_what_is_still_read(hip):
     assert out.eq(3).all() and flat[:4].eq(1).all() and flat[16:].eq(1).all()
 
 
+def captured(step):
+    """A graph of `step` and what it returned while it was recorded."""
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    return graph, out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(200, 4100, 130), (300, 5000, 1000),
+                                   (4300, 520, 1100), (1025, 8321, 2050)])
+def test_large_products_in_a_graph(hip, dtype, M, K, N):
+    """Their workspace lies in the graph's own memory: replays between eager
+    calls of the same sizes."""
+    g = gen(M)
+    X = torch.randn(M, K, generator=g).to(dtype).cuda()
+    W = hip.fp8_pack(torch.randn(K, N, generator=g).cuda())
+    graph, y = captured(lambda: hip.fp8_linear(X, W))
+    for _ in range(3):
+        X.mul_(-1.5)
+        want = hip.fp8_linear(X, W)
+        graph.replay()
+        other = hip.fp8_linear(X, W)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(other, want)
+
+
+def test_two_graphs_of_sums_that_share_memory(hip):
+    """Long bags, their join, a sort by digits and an update in place, recorded
+    twice into one pool and replayed in turn."""
+    g = gen(12)
+    V, D, n = 30000, 33, 20000
+    T, dy = torch.randn(V, D, generator=g).cuda(), torch.randn(4, D, generator=g).cuda()
+    ids = [some_ids(n, V, g) for _ in range(2)]
+    offsets = some_offsets([9000, 0, 10990, 10])
+    w = torch.rand(n, generator=g).cuda()
+
+    def step(k, table):
+        y = hip.embedding_bag(table, ids[k], offsets, w)
+        plan = hip.embedding_plan(ids[k], V, offsets)
+        hip.embedding_grad(dy, plan, w, -0.01, out=table, accumulate=True)
+        return y
+
+    eager = T.clone()
+    step(0, T.clone())
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[k], pool=pool):
+            outs.append(step(k, T))
+    for k in (0, 1, 1, 0, 1):
+        graphs[k].replay()
+        got = outs[k].clone()
+        want = step(k, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(T, eager)
+
+
 # -------------------------------------------------------------- large sizes
 def test_more_ids_than_a_launch_takes(hip):
     """2^32 threads of a launch are 2^34 rows of one column."""
