@@ -41,6 +41,7 @@ _SRC = os.path.join(_HERE, "src")
 _LIB_PATH = os.path.join(_HERE, "libkeystone_hip.so")
 
 _lib: Optional[ctypes.CDLL] = None
+_FAKE = torch._C._TorchDispatchModeKey.FAKE
 
 
 def source_files():
@@ -225,6 +226,10 @@ def gpu_ready() -> bool:
 
 
 def _stream() -> ctypes.c_void_p:
+    # what torch makes inside a FakeTensorMode has no memory, a result neither
+    if torch._C._get_dispatch_mode(_FAKE) is not None:
+        raise RuntimeError("kernels do not run on fake tensors, which have no "
+                           "memory")
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
@@ -244,12 +249,21 @@ def _launch(name: str, device: torch.device, *args) -> None:
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+    """Where t lies, for an argument that the library lets be absent."""
+    if t is None:
+        return None
+    at = t.data_ptr()
+    if not at and t.numel():
+        raise RuntimeError("a tensor without memory (a fake one, or zeros "
+                           "that torch has not made)")
+    return at
 
 
 def _check(code: int, name: str) -> None:
     if code != 0:
-        raise RuntimeError(f"{name} failed: hipError {code}")
+        # the library checks pointers itself, before any launch
+        what = " (a tensor without memory?)" if code == 1 else ""
+        raise RuntimeError(f"{name} failed: hipError {code}{what}")
 
 
 def _prep(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -257,7 +271,9 @@ def _prep(t: torch.Tensor, name: str) -> torch.Tensor:
         raise RuntimeError(f"{name}: expected CUDA tensor")
     if t.dtype != torch.float32:
         raise RuntimeError(f"{name}: expected float32, got {t.dtype}")
-    return t.contiguous()
+    t = t.contiguous()
+    _ptr(t)
+    return t
 
 
 def _prep_inplace(t: torch.Tensor, name: str) -> torch.Tensor:

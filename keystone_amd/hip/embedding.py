@@ -197,7 +197,7 @@ class EmbeddingPlan:
 
     def _places(self):
         """Where keys, order, rows and starts lie."""
-        at, step = self._kept.data_ptr(), 4 * self.n
+        at, step = _ptr(self._kept), 4 * self.n
         rows = at + 2 * step if self._bagged else at + step
         return at, at + step, rows, rows + step
 

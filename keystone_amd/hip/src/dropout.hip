@@ -94,6 +94,7 @@ KS_EXPORT int ks_dropout(const void* x, void* y, long long n, int type,
                          unsigned long long seed, unsigned long long step,
                          const long long* step_at, hipStream_t stream) {
     if (n == 0) return 0;
+    if (!x || !y) return (int)hipErrorInvalidValue;
     switch (type) {
         case 0: return dropout<float>(x, y, n, threshold, scale, seed, step, step_at, stream);
         case 1: return dropout<__bf16>(x, y, n, threshold, scale, seed, step, step_at, stream);

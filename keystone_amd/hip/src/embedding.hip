@@ -830,6 +830,7 @@ KS_EXPORT int ks_embedding_lookup(const void* ids, int ids_wide, long long n,
                                   long long ld, void* out, int D, float scale,
                                   int vec, hipStream_t stream) {
     if (n == 0 || D == 0) return 0;
+    if (!ids || !out || (V && !table)) return (int)hipErrorInvalidValue;
     const Ids t{ids, ids_wide, V};
     switch (type) {
         case F32: return lookup_by_width<float>(t, n, table, ld, out, D, scale, vec, stream);
@@ -858,6 +859,9 @@ KS_EXPORT int ks_segment_sum(int kind, const void* bounds, int fixed,
                              void* work, int D, float scale, int accumulate,
                              int vec, hipStream_t stream) {
     if (count == 0 || D == 0) return 0;
+    if (!out || (n && !ids) || (V && !src) || (kind && !bounds) ||
+        (!work && ks_segment_work(n, D, vec, keys != nullptr)))
+        return (int)hipErrorInvalidValue;
     const SumCall c{{bounds, kind, fixed, count, n},
                     {{ids, ids_wide, V}, order, weights, keys},
                     src, ld, out, ldo, work, D, scale, accumulate,

@@ -942,6 +942,7 @@ KS_EXPORT int ks_fp8_quantise(const void* x, int type, long long ld, int rows,
                               int K, unsigned char* q, unsigned char* scales,
                               hipStream_t stream) {
     if (rows == 0 || K == 0) return 0;
+    if (!x || !q || !scales) return (int)hipErrorInvalidValue;
     switch (type) {
         case 0: return quantise<float>(x, ld, rows, K, q, scales, stream);
         case 1: return quantise<__bf16>(x, ld, rows, K, q, scales, stream);
@@ -964,6 +965,8 @@ KS_EXPORT int ks_fp8_linear(const void* x, int type, long long ld,
                             unsigned char* work, hipStream_t stream) {
     if (M == 0 || N == 0) return 0;
     const Work w = work_of(type, M, K, N);
+    if (!x || !wq || !ws || !y || (w.bytes && !work))
+        return (int)hipErrorInvalidValue;
     if (w.quantised) {
         const int code = ks_fp8_quantise(x, type, ld, M, K, work,
                                          work + w.scales, stream);

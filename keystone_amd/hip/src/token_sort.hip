@@ -533,6 +533,9 @@ KS_EXPORT int ks_token_sort(const void* ids, int ids_wide, int n, int V,
                             int kind, const void* bounds, int fixed, int bags,
                             int* keys, int* order, int* rows, int* starts,
                             int* work, hipStream_t stream) {
+    if (!starts || (n && (!ids || !keys || !order)) || (kind && !bounds) ||
+        (!work && ks_token_sort_work(n, V)))
+        return (int)hipErrorInvalidValue;
     const Bags segments{bounds, kind, fixed, bags};
     if (n > 0 && n <= SMALL) {
         const int placing = ks_ceil_div(n, PLACED);

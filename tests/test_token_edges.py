@@ -189,3 +189,44 @@ def test_means_of_64_bit_tables_are_in_64_bits():
     S = want @ params[1] + params[2]
     ref = torch.nn.functional.cross_entropy(S, torch.tensor([0, 1, 2]))
     assert abs(loss.item() - ref.item()) < 1e-14
+
+
+@pytest.mark.skipif(not hip.available(), reason="extension not built")
+def test_the_library_refuses_absent_memory():
+    """Pointers that have to be there are checked before any launch: 1 is an
+    invalid argument."""
+    lib = hip._load()
+    some = torch.zeros(4096, dtype=torch.uint8)
+    p = some.data_ptr()
+
+    def refused(name, args, absent):
+        for i in absent:
+            bad = list(args)
+            assert bad[i] == p
+            bad[i] = None
+            assert getattr(lib, name)(*bad) == 1, (name, i)
+
+    refused("ks_embedding_lookup", [p, 0, 3, p, 0, 5, 8, p, 8, 1.0, 4, None],
+            (0, 3, 7))
+    refused("ks_segment_sum", [1, p, 0, 2, 3, p, 0, 5, None, None, None, p, 0, 8,
+                               p, 0, 8, None, 8, 1.0, 0, 4, None], (1, 5, 11, 14))
+    refused("ks_segment_sum", [0, None, 9000, 1, 9000, p, 0, 5, None, None, None,
+                               p, 0, 8, p, 0, 8, p, 8, 1.0, 0, 4, None], (17,))
+    refused("ks_token_sort", [p, 0, 3, 5, 1, p, 0, 2, p, p, p, p, None, None],
+            (0, 5, 8, 9, 11))
+    refused("ks_token_sort", [p, 0, 9000, 5, 0, None, 1, 9000, p, p, None, p, p,
+                              None], (12,))
+    refused("ks_dropout", [p, p, 9, 0, 5, 1.0, 1, 2, None, None], (0, 1))
+    refused("ks_fp8_quantise", [p, 0, 5, 3, 5, p, p, None], (0, 5, 6))
+    refused("ks_fp8_linear", [p, 0, 5, p, p, None, p, 3, 5, 7, None, None],
+            (0, 3, 4, 6))
+    refused("ks_fp8_linear", [p, 0, 9000, p, p, None, p, 64, 9000, 700, p, None],
+            (10,))
+
+
+def test_no_kernel_runs_in_a_mode_of_fake_tensors():
+    """Its results would have no memory either: refused before the launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        with pytest.raises(RuntimeError, match="memory"):
+            hip._stream()

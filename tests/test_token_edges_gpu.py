@@ -311,6 +311,58 @@ def test_two_graphs_of_sums_that_share_memory(hip):
         assert torch.equal(got, want) and torch.equal(T, eager)
 
 
+def test_tensors_without_memory_are_refused(hip):
+    """Fake tensors and zeros that torch has not made have no address: nothing
+    is launched for them, not for one of several arguments either."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    real = dict(T=torch.ones(6, 8, device="cuda"), w=torch.ones(5, device="cuda"),
+                ids=torch.arange(5, device="cuda"),
+                off=torch.tensor([0, 2, 5], device="cuda"),
+                dy=torch.ones(2, 8, device="cuda"), b=torch.ones(3, device="cuda"),
+                step=torch.ones(1, dtype=torch.int64, device="cuda"),
+                X=torch.ones(4, 6, device="cuda"), W=torch.ones(6, 3, device="cuda"))
+    plan = hip.embedding_plan(real["ids"], 6, real["off"])
+    packed = hip.fp8_pack(real["W"])
+    calls = {
+        ("T", "ids"): lambda T, ids, **k: hip.embedding_lookup(T, ids),
+        ("T", "ids", "off", "w"): lambda T, ids, off, w, **k:
+            hip.embedding_bag(T, ids, off, w),
+        ("ids", "off"): lambda ids, off, **k: hip.embedding_plan(ids, 6, off),
+        ("dy", "w"): lambda dy, w, **k: hip.embedding_grad(dy, plan, w),
+        ("X", "step"): lambda X, step, **k: hip.dropout(X, 0.5, 1, step),
+        ("W",): lambda W, **k: hip.fp8_pack(W),
+        ("X", "b"): lambda X, b, **k: hip.fp8_linear(X, packed, b),
+    }
+    for names, call in calls.items():
+        call(**real)
+        for name in names:
+            # zeros of a call that copies its argument are made by the copy
+            zero = torch._efficientzerotensor(
+                real[name].shape, dtype=real[name].dtype, device="cuda")
+            try:
+                got = call(**{**real, name: zero})
+            except RuntimeError as e:
+                assert "memory" in str(e), e
+            else:
+                want = call(**{**real, name: zero.clone()})
+                if isinstance(want, torch.Tensor):
+                    assert torch.equal(got, want)
+                else:
+                    assert all(torch.equal(u, v) for u, v in zip(
+                        vars(got).values(), vars(want).values())
+                        if isinstance(u, torch.Tensor))
+            with FakeTensorMode():
+                fake = torch.empty(real[name].shape, dtype=real[name].dtype,
+                                   device="cuda")
+            with pytest.raises(RuntimeError, match="memory"):
+                call(**{**real, name: fake})
+        # a mode that makes every result a fake one takes no real argument
+        with FakeTensorMode():
+            with pytest.raises((RuntimeError, AssertionError)):
+                call(**real)
+    torch.cuda.synchronize()
+
+
 # -------------------------------------------------------------- large sizes
 def test_more_ids_than_a_launch_takes(hip):
     """2^32 threads of a launch are 2^34 rows of one column."""
