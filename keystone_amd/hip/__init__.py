@@ -271,7 +271,7 @@ def _prep(t: torch.Tensor, name: str) -> torch.Tensor:
         raise RuntimeError(f"{name}: expected CUDA tensor")
     if t.dtype != torch.float32:
         raise RuntimeError(f"{name}: expected float32, got {t.dtype}")
-    t = t.contiguous()
+    t = t.resolve_neg().contiguous()
     _ptr(t)
     return t
 
@@ -279,9 +279,9 @@ def _prep(t: torch.Tensor, name: str) -> torch.Tensor:
 def _prep_inplace(t: torch.Tensor, name: str) -> torch.Tensor:
     """For in-place kernels: a silent .contiguous() copy would leave the
     caller's tensor unmodified — fail loudly on layout regressions."""
-    if not t.is_contiguous():
+    if not t.is_contiguous() or t.is_neg():
         raise RuntimeError(f"{name}: in-place kernel needs a contiguous "
-                           "tensor (got a strided view)")
+                           "tensor (got a strided or negated view)")
     return _prep(t, name)
 
 

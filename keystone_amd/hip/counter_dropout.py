@@ -53,14 +53,17 @@ def dropout(x: torch.Tensor, p: float, seed: int,
         at, step = step, 0
     elif not 0 <= step < 2 ** 64:
         raise ValueError(f"dropout: expected a step in [0, 2^64), got {step}")
+    if x.is_neg():                # a sign that torch has put off
+        x = x.resolve_neg()
     if out is None:
         x = x.contiguous()
         out = torch.empty_like(x)
     else:
         if out.shape != x.shape or out.dtype != x.dtype \
-                or out.device != x.device or not out.is_contiguous():
+                or out.device != x.device or not out.is_contiguous() \
+                or out.is_neg():
             raise RuntimeError("dropout.out: expected a contiguous tensor of "
-                               "x's shape, type and device")
+                               "x's shape, type and device, no negated view")
         x = x.contiguous()
         lo, size = out.data_ptr(), x.numel() * x.element_size()
         if 0 < abs(x.data_ptr() - lo) < size:

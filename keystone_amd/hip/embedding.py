@@ -46,6 +46,8 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     if rows > _MAX_ROWS or D > _MAX_DIM:
         raise ValueError(f"{name}: {tuple(t.shape)} is over {_MAX_ROWS} rows "
                          f"or {_MAX_DIM} columns")
+    if t.is_neg():                # a sign that torch has put off
+        t = t.resolve_neg()
     if D > 1 and t.stride(1) != 1:
         return t.contiguous()
     return t
@@ -68,6 +70,8 @@ def _weights(w: Optional[torch.Tensor], n: int, name: str, device):
                            f"{w.dtype} on {w.device}")
     if w.numel() != n:
         raise ValueError(f"{name}: {w.numel()} weights for {n} ids")
+    if w.is_neg():
+        w = w.resolve_neg()
     return w.contiguous()
 
 
@@ -293,9 +297,10 @@ def embedding_grad(grad: torch.Tensor, plan: EmbeddingPlan,
                                f"bfloat16 or float16 on {grad.device}, got "
                                f"{out.dtype} on {out.device}")
         if (out.shape[1] > 1 and out.stride(1) != 1) or \
-                (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+                (out.shape[0] > 1 and out.stride(0) < out.shape[1]) \
+                or out.is_neg():
             raise RuntimeError("embedding_grad.out: rows must be contiguous "
-                               "and apart")
+                               "and apart, and no negated view")
         if out.numel() and grad.numel():
             a, b = _span(out)
             read = {"grad": _span(grad)}

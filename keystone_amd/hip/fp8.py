@@ -103,6 +103,8 @@ def _operand(x: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name}: expected a matrix with at most "
                          f"{_MAX_INNER} of the inner dimension and {_MAX} of "
                          f"the other, got shape {tuple(x.shape)}")
+    if x.is_neg():                # a sign that torch has put off
+        x = x.resolve_neg()
     return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
 
 
@@ -169,7 +171,7 @@ def fp8_linear(X: torch.Tensor, W: Fp8Weight,
         if bias.shape != (W.N,):
             raise ValueError(f"fp8_linear.bias: expected shape ({W.N},), got "
                              f"{tuple(bias.shape)}")
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     out = X.new_empty((M, W.N))
     if M == 0 or W.N == 0:
         return out

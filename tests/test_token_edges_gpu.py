@@ -311,6 +311,47 @@ def test_two_graphs_of_sums_that_share_memory(hip):
         assert torch.equal(got, want) and torch.equal(T, eager)
 
 
+def test_negated_views(hip):
+    """The imaginary part of a conjugate is a view whose sign torch puts off:
+    its memory holds the opposite."""
+    g = gen(13)
+
+    def negated(*shape):
+        z = torch.randn(*shape, 2, generator=g).cuda()
+        n = torch.view_as_complex(z).conj().imag
+        assert n.is_neg() and torch.equal(n, -z[..., 1])
+        return n
+
+    ids = some_ids(60, 9, g)
+    plan = hip.embedding_plan(ids, 9)
+    X, W, b = negated(7, 200), negated(200, 5), negated(5)
+    for D in (1, 6):
+        for T in (negated(9, D), torch._neg_view(torch.randn(9, D, generator=g).cuda())):
+            real = T.clone()
+            assert not real.is_neg()
+            for f in (lambda t: hip.embedding_lookup(t, ids),
+                      lambda t: hip.embedding_bag(t, ids.view(6, 10)),
+                      lambda t: hip.dropout(t, 0.3, 1, 2),
+                      lambda t: hip.sym_rectify(t),
+                      lambda t: hip.fp8_pack(t).dequantise()):
+                assert torch.equal(f(T), f(real))
+    for dy in (negated(60, 3), negated(60, 1)):
+        w = negated(60)
+        assert torch.equal(hip.embedding_grad(dy, plan, w),
+                           hip.embedding_grad(dy.clone(), plan, w.clone()))
+    packed = hip.fp8_pack(W)
+    assert torch.equal(hip.fp8_linear(X, packed, b),
+                       hip.fp8_linear(X.clone(), hip.fp8_pack(W.clone()), b.clone()))
+    one = negated(7, 1)
+    thin = hip.fp8_pack(torch.ones(1, 3, device="cuda"))
+    assert torch.equal(hip.fp8_linear(one, thin), hip.fp8_linear(one.clone(), thin))
+    out = torch._neg_view(torch.ones(9, 3, device="cuda"))
+    with pytest.raises(RuntimeError, match="negated"):
+        hip.embedding_grad(torch.ones(60, 3, device="cuda"), plan, out=out)
+    with pytest.raises(RuntimeError, match="negated"):
+        hip.dropout(torch.ones(9, 3, device="cuda"), 0.5, 1, out=out)
+
+
 def test_tensors_without_memory_are_refused(hip):
     """Fake tensors and zeros that torch has not made have no address: nothing
     is launched for them, not for one of several arguments either."""
